@@ -262,15 +262,15 @@ def _plain_attention(s):
 def _own(s):
     c = s["case"]
     if c["op"] == "norm":
-        from pixelsplat_amd.group_norm import group_norm
+        from pixelsplat_amd.ops import group_norm
         leaves = [s["x"], s["weight"], s["bias"]]
         y = group_norm(s["x"], c["groups"], s["weight"], s["bias"], eps=EPS, activation=c["act"])
     elif c["op"] == "gated":
-        from pixelsplat_amd.gated_linear import gated_linear
+        from pixelsplat_amd.ops import gated_linear
         leaves = [s["x"], s["w_gate"], s["w_up"]] + ([s["b_gate"], s["b_up"]] if c["bias"] else [])
         y = gated_linear(s["x"], s["w_gate"], s["w_up"], s["b_gate"], s["b_up"], activation=c["act"])
     else:
-        from pixelsplat_amd.relative_attention import relative_attention
+        from pixelsplat_amd.ops import relative_attention
         leaves = [s["q"], s["k"], s["v"], s["table"]]
         y = relative_attention(s["q"], s["k"], s["v"], s["table"], s["buckets"], key_mask=s["mask"],
                                query_start=s["start"])
