@@ -1,0 +1,80 @@
+// Element types of the operators that take fp32, bf16 and fp16 tensors: 16-byte vectors of them, conversion to
+// and from the fp32 all arithmetic is done in, and the activations with their slopes.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace ps {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+// V elements moved as one 4*V- or 2*V-byte access
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Pack { T v[V]; };
+
+template <typename T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }
+template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }   // round to nearest even
+
+// parameters are stored in the tensors' type or in fp32
+template <typename T>
+__device__ __forceinline__ float load_param(const void* p, int is_f32, int64_t i) {
+  return is_f32 ? reinterpret_cast<const float*>(p)[i] : to_f32(reinterpret_cast<const T*>(p)[i]);
+}
+template <typename T>
+__device__ __forceinline__ void store_param(void* p, int is_f32, int64_t i, float v) {
+  if (is_f32) reinterpret_cast<float*>(p)[i] = v;
+  else reinterpret_cast<T*>(p)[i] = from_f32<T>(v);
+}
+
+// 0.5 (1 + erf(z / sqrt 2)) and exp(-z^2 / 2).  fp32 tensors use erff.  16-bit tensors use the rational form
+// 7.1.26 of Abramowitz & Stegun, erf(x) = 1 - t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + p x): its absolute error
+// of 1.5e-7 is far below half a step of the result's type, it shares the exponential with the slope, and it is a
+// third of the instructions.
+template <bool EXACT>
+__device__ __forceinline__ void normal_cdf(float z, float& cdf, float& bell) {
+  bell = __expf(-0.5f * z * z);
+  if (EXACT) {
+    cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+  } else {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f),
+                                       -0.284496736f), 0.254829592f);
+    const float tail = 0.5f * poly * bell;
+    cdf = z < 0.f ? tail : 1.f - tail;
+  }
+}
+__device__ __forceinline__ float sigmoid_f32(float z) { return 1.f / (1.f + __expf(-z)); }
+
+// the PS_ACT_ values of pixelsplat_ops.h
+enum Act { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_SIGMOID = 4 };
+
+template <bool EXACT>
+__device__ __forceinline__ float act_value(int act, float z) {
+  switch (act) {
+    case ACT_RELU: return z > 0.f || z != z ? z : 0.f;
+    case ACT_SILU: return z * sigmoid_f32(z);
+    case ACT_GELU: { float cdf, bell; normal_cdf<EXACT>(z, cdf, bell); return z * cdf; }
+    case ACT_SIGMOID: return sigmoid_f32(z);
+    default: return z;
+  }
+}
+// act'(z); *value = act(z)
+template <bool EXACT>
+__device__ __forceinline__ float act_slope(int act, float z, float* value) {
+  switch (act) {
+    case ACT_RELU: *value = z > 0.f || z != z ? z : 0.f; return z > 0.f ? 1.f : 0.f;
+    case ACT_SILU: { const float s = sigmoid_f32(z); *value = z * s; return s * fmaf(z, 1.f - s, 1.f); }
+    case ACT_GELU: {
+      float cdf, bell;
+      normal_cdf<EXACT>(z, cdf, bell);
+      *value = z * cdf;
+      return fmaf(z * 0.39894228040143268f, bell, cdf);
+    }
+    case ACT_SIGMOID: { const float s = sigmoid_f32(z); *value = s; return s * (1.f - s); }
+    default: *value = z; return 1.f;
+  }
+}
+
+}  // namespace ps

@@ -1,0 +1,58 @@
+/*
+ * pixelsplat_ops.h -- C ABI of libpixelsplat_ops.so (MI355X / gfx950): the operators of image-transformer blocks.
+ *
+ * The conventions are those of pixelsplat_hip.h: plain pointers and sizes, every buffer is DEVICE memory owned by the
+ * caller, `stream` is a hipStream_t passed as void*, the library keeps no state between calls, never throws, aborts or
+ * synchronises, and returns 0 or a negative PsStatus.  Launches go to the calling thread's current device, which has to
+ * be the tensors' own.
+ *
+ * Tensors have one of three element types; arithmetic is fp32 (sums over many elements fp32 or fp64), results are
+ * rounded to nearest even.  All of it is deterministic: the same inputs give the same bits.
+ */
+#ifndef PIXELSPLAT_OPS_H
+#define PIXELSPLAT_OPS_H
+
+#include "pixelsplat_hip.h" /* PsStatus */
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define PS_DTYPE_F32 0
+#define PS_DTYPE_BF16 1
+#define PS_DTYPE_F16 2
+
+#define PS_ACT_NONE 0
+#define PS_ACT_RELU 1
+#define PS_ACT_SILU 2 /* z sigmoid(z)                 */
+#define PS_ACT_GELU 3 /* z (1 + erf(z / sqrt 2)) / 2  */
+#define PS_ACT_SIGMOID 4
+
+/* Group norm with an activation, channels last: x [samples][rows][channels] (unit channel stride, strides of samples
+ * and rows in elements), y = act((x - mean) rstd gamma + beta) with mean and variance over the rows and the
+ * channels / groups channels of a (sample, group); y and dx are contiguous and 16-byte aligned.  gamma, beta
+ * [channels] in the tensors' type, or fp32 when param_f32; either may be NULL (1 and 0).  mean, rstd [samples][groups]
+ * fp32 are what the backward needs of the forward.  d_gamma / d_beta are in the parameters' type, NULL when not
+ * wanted.  channels <= 8192, samples <= 65535, rows * channels < 2^31 (else PS_ERR_UNSUPPORTED).
+ * workspace: ps_group_norm_workspace_bytes(desc, backward) bytes, 16-byte aligned, its contents are not kept. */
+typedef struct PsGroupNormDesc {
+  int32_t samples, rows, channels, groups;
+  int32_t dtype, activation, param_f32;
+  float eps;
+  int64_t x_sample_stride, x_row_stride;
+  int64_t dy_sample_stride, dy_row_stride; /* backward only */
+} PsGroupNormDesc;
+size_t ps_group_norm_workspace_bytes(const PsGroupNormDesc* desc, int32_t backward);
+int ps_group_norm_forward(const PsGroupNormDesc* desc, const void* x, const void* gamma, const void* beta, void* y,
+                          float* mean, float* rstd, void* workspace, size_t workspace_bytes, void* stream);
+int ps_group_norm_backward(const PsGroupNormDesc* desc, const void* x, const void* dy, const void* gamma,
+                           const void* beta, const float* mean, const float* rstd, void* dx, void* d_gamma,
+                           void* d_beta, void* workspace, size_t workspace_bytes, void* stream);
+
+/* "pixelsplat_ops gfx950 | <file>:<hash> ...", as ps_build_info of pixelsplat_hip.h. */
+const char* ps_ops_build_info(void);
+
+#ifdef __cplusplus
+}
+#endif
+#endif
