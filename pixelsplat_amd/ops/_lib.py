@@ -25,13 +25,21 @@ class PsGroupNormDesc(C.Structure):
         (n, C.c_int64) for n in ("x_sample_stride", "x_row_stride", "dy_sample_stride", "dy_row_stride")]
 
 
+class PsGatedLinearDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("rows", "dim", "hidden", "dtype", "activation", "reserved")] + [
+        (n, C.c_int64) for n in ("x_row_stride", "w_row_stride", "dh_row_stride")]
+
+
 _vp, _size, _i32 = C.c_void_p, C.c_size_t, C.c_int32
-_pn = C.POINTER(PsGroupNormDesc)
+_pn, _pg = C.POINTER(PsGroupNormDesc), C.POINTER(PsGatedLinearDesc)
 # every symbol pixelsplat_ops.h declares: (result, arguments)
 SIGNATURES = {
     "ps_group_norm_workspace_bytes": (_size, [_pn, _i32]),
     "ps_group_norm_forward": (C.c_int, [_pn] + [_vp] * 7 + [_size, _vp]),
     "ps_group_norm_backward": (C.c_int, [_pn] + [_vp] * 10 + [_size, _vp]),
+    "ps_gated_linear_forward": (C.c_int, [_pg] + [_vp] * 9),
+    "ps_gated_linear_backward_workspace_bytes": (_size, [_pg]),
+    "ps_gated_linear_backward": (C.c_int, [_pg] + [_vp] * 14 + [_size, _vp]),
     "ps_ops_build_info": (C.c_char_p, []),
 }
 

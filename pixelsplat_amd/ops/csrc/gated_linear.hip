@@ -1,0 +1,592 @@
+// Gated projection of a feed-forward block, h = act(x Wg^T + bg) * (x Wu^T + bu), and its backward pass
+//   du = dh act(a), da = dh u act'(a)   (a, u the two projections)
+//   dx = da Wg + du Wu;  dWg = da^T x;  dWu = du^T x;  dbg, dbu = column sums of da, du.
+//
+// Bound by the matrix instructions (4 M D F flop forward, 8 M D F backward), except for a few rows, where the two
+// weight matrices are all there is to read.
+//
+// One tiled product serves all of it.  A block computes a BM x BN tile; both operands go from global memory straight
+// into LDS in slices of 128 bytes of the contraction index, double buffered, and from there as MFMA fragments.
+// Operands lie along the contraction index (x, W in the forward) or across it (W in dx, both in dW: transposing LDS
+// reads, no copies).  In the forward a block's columns are gate and up columns of the same hidden units in
+// alternating runs of 32, so that the wave that holds a also holds u and the activation is its epilogue: neither
+// projection reaches memory.
+//
+// What the backward needs of a and u: fp32 tensors keep both (8 bytes a hidden value, against 4 D flop at 150
+// TFLOP/s); 16-bit tensors compute them again (the products are 8 times as fast, and keeping them rounded to 16 bits
+// would put a second rounding into every gradient).  da and du are rounded to the tensors' type before they enter
+// their products, as h is before its own.
+#include "mfma_tile.h"
+#include "pixelsplat_ops.h"
+
+namespace ps {
+namespace {
+
+__device__ const uint4 kZeros[1] = {{0, 0, 0, 0}};   // what a copy reads for a chunk outside its operand
+
+constexpr int kSliceBytes = 128;
+
+struct Operand {
+  const void* p[2];       // two matrices: the halves of the contraction (dx), or of the columns (forward)
+  int64_t ld;             // elements
+};
+
+struct Product {
+  int m, n, k;            // n: columns of the result (forward: hidden units); k: of one half
+  int halves;             // of the contraction index
+  Operand a, b;
+  int tiles_m, tiles_n, splits, slices_per_split;
+};
+
+// which columns of a forward block belong to which projection
+__device__ __forceinline__ int pair_unit(int col) { return (col >> 6) * 32 + (col & 31); }
+__device__ __forceinline__ int pair_half(int col) { return (col >> 5) & 1; }
+
+// blocks go to the 8 dies in turn: each die gets a run of neighbouring tiles, and its L2 the operands they share
+__device__ __forceinline__ int die_order(int id, int count) {
+  const int per = count >> 3, extra = count & 7, die = id & 7, at = id >> 3;
+  return die * per + min(die, extra) + at;
+}
+
+// A copier owns what a wave copies of one operand: kPieces pieces of 1 KB of its tile every slice.
+template <typename T, int ROWS, int WAVES, bool ACROSS>
+struct Copier {
+  static constexpr int kPieces = ROWS * kSliceBytes / 1024 / WAVES;
+  const T* at[kPieces];     // at contraction index 0; NULL: outside the operand
+  int kk[kPieces];          // contraction index within the slice
+  int64_t other, step;      // from the first matrix to the second; elements of a contraction index
+
+  template <bool PAIRED>
+  __device__ __forceinline__ void init(const Operand& o, int row0, int rows, int wave, int lane) {
+    const T* p0 = reinterpret_cast<const T*>(o.p[0]);
+    const T* p1 = reinterpret_cast<const T*>(o.p[1]);
+    other = (reinterpret_cast<const char*>(p1) - reinterpret_cast<const char*>(p0)) / (int)sizeof(T);
+    step = ACROSS ? o.ld : 1;
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
+      const int piece = j * WAVES + wave, pos = piece * 64 + lane;
+      if (ACROSS) {
+        constexpr int kChunks = ROWS / kVec<T>;                  // of a row of the tile
+        const int k = pos / kChunks;
+        const int row = row0 + ((pos % kChunks) ^ across_swizzle<T>(k)) * kVec<T>;
+        at[j] = row < rows ? p0 + k * o.ld + row : nullptr;
+        kk[j] = k;
+      } else {
+        const int r = pos >> 3, chunk = (pos & 7) ^ ((r >> 1) & 7);
+        const int row = PAIRED ? row0 / 2 + pair_unit(r) : row0 + r;
+        at[j] = row < rows ? (PAIRED && pair_half(piece * 8) ? p1 : p0) + row * o.ld + chunk * kVec<T> : nullptr;
+        kk[j] = chunk * kVec<T>;
+      }
+    }
+  }
+  // slice [k0, ...) of a contraction of length k, in the first or second matrix
+  __device__ __forceinline__ void copy(int which, int k0, int k, char* tile, int wave) const {
+    const int64_t delta = k0 * step + (which ? other : 0);
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
+      const bool inside = at[j] != nullptr && k0 + kk[j] < k;
+      copy_to_lds(inside ? (const void*)(at[j] + delta) : (const void*)kZeros, tile + (j * WAVES + wave) * 1024);
+    }
+  }
+};
+
+// BM x BN tile of WM x WN waves; EP(acc, row, column of the wave's tile) writes the result
+template <typename T, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, bool PAIRED, typename EP>
+__global__ void __launch_bounds__(WM * WN * 64, 2)
+product_kernel(Product g, EP ep) {
+  constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, kK = kSliceBytes / sizeof(T);
+  constexpr int kA = BM * kSliceBytes, kB = BN * kSliceBytes;
+  extern __shared__ __attribute__((aligned(16))) char lds[];    // 2 x (A | B)
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, hi = lane >> 5;
+  const int wm = wave / WN, wn = wave % WN;
+  // tiles of 8 rows of tiles at a time, column by column: neighbours share their operands in the die's L2
+  const int id = die_order(blockIdx.x, g.tiles_m * g.tiles_n);
+  const int group = id / (8 * g.tiles_n), rows_in = min(8, g.tiles_m - group * 8), in = id - group * 8 * g.tiles_n;
+  const int tm = group * 8 + in % rows_in, tn = in / rows_in;
+  const int m0 = tm * BM, n0 = tn * BN;
+
+  Copier<T, BM, WAVES, A_ACROSS> ca;
+  Copier<T, BN, WAVES, B_ACROSS> cb;
+  ca.template init<false>(g.a, m0, g.m, wave, lane);
+  cb.template init<PAIRED>(g.b, n0, g.n, wave, lane);
+
+  floatx16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = zero16();
+
+  const int per_half = (g.k + kK - 1) / kK, slices = per_half * g.halves;
+  const int s0 = blockIdx.y * g.slices_per_split, s1 = min(s0 + g.slices_per_split, slices);
+  auto load = [&](int s, int buf) {
+    const int which = s >= per_half ? 1 : 0, k0 = (s - which * per_half) * kK;
+    ca.copy(which, k0, g.k, lds + buf * (kA + kB), wave);
+    cb.copy(which, k0, g.k, lds + buf * (kA + kB) + kA, wave);
+  };
+  if (s0 < s1) load(s0, 0);
+  __syncthreads();
+  for (int s = s0; s < s1; ++s) {
+    const int buf = (s - s0) & 1;
+    if (s + 1 < s1) load(s + 1, buf ^ 1);
+    const char* ta = lds + buf * (kA + kB);
+    const char* tb = ta + kA;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {                    // 32 bytes of the contraction index a step
+      Frag<T> fa[TM], fb[TN];
+      const int k0 = (2 * c + hi) * kVec<T>;
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int row = (wm * TM + i) * 32;
+        fa[i] = A_ACROSS ? across_fragment<T, BM>(ta, row, k0, k0 + 4, lane)
+                         : along_fragment<T>(ta, row + (lane & 31), 2 * c + hi);
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int row = (wn * TN + j) * 32;
+        fb[j] = B_ACROSS ? across_fragment<T, BN>(tb, row, k0, k0 + 4, lane)
+                         : along_fragment<T>(tb, row + (lane & 31), 2 * c + hi);
+      }
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = mfma(fa[i], fb[j], acc[i][j]);
+    }
+    __syncthreads();                                 // the next slice has arrived, this one has been read
+  }
+  ep.template store<T, TM, TN>(acc, m0 + wm * TM * 32, n0 + wn * TN * 32, lane, g, tm * WM + wm);
+}
+
+// ---- epilogues --------------------------------------------------------------------------------------------------
+// h, and (fp32 training) a and u
+struct StoreGated {
+  void* h;
+  const void *bg, *bu;
+  float *a, *u;           // NULL: not kept
+  int act;
+  template <typename T, int TM, int TN>
+  __device__ __forceinline__ void store(const floatx16 (&acc)[TM][TN], int row0, int col0, int lane, const Product& g, int) {
+#pragma unroll
+    for (int j = 0; j < TN; j += 2) {
+      const int f = (col0 + j * 32) / 2 + (lane & 31);
+      if (f >= g.n) continue;
+      const float wg = bg ? to_f32(reinterpret_cast<const T*>(bg)[f]) : 0.f;
+      const float wu = bu ? to_f32(reinterpret_cast<const T*>(bu)[f]) : 0.f;
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = row0 + i * 32 + result_row(r, lane >> 5);
+          if (row >= g.m) continue;
+          const float za = acc[i][j][r] + wg, zu = acc[i][j + 1][r] + wu;
+          const int64_t at = (int64_t)row * g.n + f;
+          reinterpret_cast<T*>(h)[at] = from_f32<T>(act_value<sizeof(T) == 4>(act, za) * zu);
+          if (a) { a[at] = za; u[at] = zu; }
+        }
+    }
+  }
+};
+
+// da and du from the recomputed projections; with biases, their column sums over the wave's rows
+struct StoreGatedGrad {
+  const void* dh;
+  int64_t ld_dh;
+  const void *bg, *bu;
+  void *da, *du;          // [m][ld]
+  int ld;
+  float* sums;            // [row parts][2][ld] or NULL
+  int act;
+  template <typename T, int TM, int TN>
+  __device__ __forceinline__ void store(const floatx16 (&acc)[TM][TN], int row0, int col0, int lane, const Product& g,
+                                        int row_part) {
+#pragma unroll
+    for (int j = 0; j < TN; j += 2) {
+      const int f = (col0 + j * 32) / 2 + (lane & 31);
+      if (f >= ld) continue;
+      const bool on = f < g.n;                          // the columns behind the last are zero
+      const float wg = on && bg ? to_f32(reinterpret_cast<const T*>(bg)[f]) : 0.f;
+      const float wu = on && bu ? to_f32(reinterpret_cast<const T*>(bu)[f]) : 0.f;
+      float sa = 0.f, su = 0.f;
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = row0 + i * 32 + result_row(r, lane >> 5);
+          if (row >= g.m) continue;
+          float va = 0.f, vu = 0.f;
+          if (on) {
+            const float d = to_f32(reinterpret_cast<const T*>(dh)[row * ld_dh + f]);
+            float value;
+            const float slope = act_slope<sizeof(T) == 4>(act, acc[i][j][r] + wg, &value);
+            va = d * (acc[i][j + 1][r] + wu) * slope;
+            vu = d * value;
+          }
+          const int64_t at = (int64_t)row * ld + f;
+          reinterpret_cast<T*>(da)[at] = from_f32<T>(va);
+          reinterpret_cast<T*>(du)[at] = from_f32<T>(vu);
+          sa += va;
+          su += vu;
+        }
+      if (sums) {
+        sa += __shfl_xor(sa, 32);
+        su += __shfl_xor(su, 32);
+        if (lane < 32) {
+          sums[((int64_t)row_part * 2 + 0) * ld + f] = sa;
+          sums[((int64_t)row_part * 2 + 1) * ld + f] = su;
+        }
+      }
+    }
+  }
+};
+
+// the product itself, or this split's part of it in fp32
+struct StoreMatrix {
+  void* c;
+  float* parts;           // [splits][m][n] or NULL
+  template <typename T, int TM, int TN>
+  __device__ __forceinline__ void store(const floatx16 (&acc)[TM][TN], int row0, int col0, int lane, const Product& g, int) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int col = col0 + j * 32 + (lane & 31);
+      if (col >= g.n) continue;
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = row0 + i * 32 + result_row(r, lane >> 5);
+          if (row >= g.m) continue;
+          if (parts) parts[((int64_t)blockIdx.y * g.m + row) * g.n + col] = acc[i][j][r];
+          else reinterpret_cast<T*>(c)[(int64_t)row * g.n + col] = from_f32<T>(acc[i][j][r]);
+        }
+    }
+  }
+};
+
+// ---- small kernels ----------------------------------------------------------------------------------------------
+// c = sum of the parts, in their order
+template <typename T>
+__global__ void __launch_bounds__(256) join_parts_kernel(int64_t count, int splits, const float* __restrict__ parts,
+                                                         T* __restrict__ c) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= count) return;
+  float t = 0.f;
+  for (int s = 0; s < splits; ++s) t += parts[s * count + i];
+  c[i] = from_f32<T>(t);
+}
+
+// fp32: da, du of the kept projections.  A block takes `rows` rows of 256 columns and leaves their column sums.
+__global__ void __launch_bounds__(256) gated_slope_kernel(int m, int n, int ld, int rows, int act, const float* __restrict__ a,
+                                                          const float* __restrict__ u, const float* __restrict__ dh,
+                                                          int64_t ld_dh, float* __restrict__ da, float* __restrict__ du,
+                                                          float* __restrict__ sums) {
+  const int f = blockIdx.x * 256 + threadIdx.x;
+  if (f >= ld) return;
+  const int r0 = blockIdx.y * rows, r1 = min(r0 + rows, m);
+  float sa = 0.f, su = 0.f;
+#pragma unroll 4
+  for (int r = r0; r < r1; ++r) {
+    float va = 0.f, vu = 0.f;
+    if (f < n) {
+      const float d = dh[r * ld_dh + f];
+      float value;
+      const float slope = act_slope<true>(act, a[(int64_t)r * n + f], &value);
+      va = d * u[(int64_t)r * n + f] * slope;
+      vu = d * value;
+    }
+    da[(int64_t)r * ld + f] = va;
+    du[(int64_t)r * ld + f] = vu;
+    sa += va;
+    su += vu;
+  }
+  if (sums) {
+    sums[((int64_t)blockIdx.y * 2 + 0) * ld + f] = sa;
+    sums[((int64_t)blockIdx.y * 2 + 1) * ld + f] = su;
+  }
+}
+
+// dbg | dbu: 16 columns a block, 16 threads a column, the parts in order
+template <typename T>
+__global__ void __launch_bounds__(256) gated_bias_kernel(int parts, int n, int ld, const float* __restrict__ sums,
+                                                         T* __restrict__ dbg, T* __restrict__ dbu) {
+  __shared__ double lds[16][17];
+  const int col = blockIdx.x * 16 + (threadIdx.x & 15), l = threadIdx.x >> 4;
+  double t = 0;
+  if (col < 2 * ld)
+    for (int p = l; p < parts; p += 16) t += sums[(int64_t)p * 2 * ld + col];
+  lds[l][threadIdx.x & 15] = t;
+  __syncthreads();
+  if (l == 0 && col < 2 * ld) {
+    for (int k = 1; k < 16; ++k) t += lds[k][threadIdx.x];
+    const int f = col < ld ? col : col - ld;
+    T* out = col < ld ? dbg : dbu;
+    if (out && f < n) out[f] = from_f32<T>((float)t);
+  }
+}
+
+// ---- a few rows: a wave takes a hidden unit, its lanes the contraction index --------------------------------------
+template <typename T, int M>
+__global__ void __launch_bounds__(256) gated_rows_kernel(int m, int d, int n, int act, const T* __restrict__ x, int64_t ldx,
+                                                         const T* __restrict__ wg, const T* __restrict__ wu, int64_t ldw,
+                                                         const T* __restrict__ bg, const T* __restrict__ bu, T* __restrict__ h,
+                                                         float* __restrict__ a, float* __restrict__ u) {
+  const int f = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (f >= n) return;
+  constexpr int V = kVec<T>;
+  float sa[M], su[M];
+#pragma unroll
+  for (int i = 0; i < M; ++i) sa[i] = su[i] = 0.f;
+  const T* rg = wg + f * ldw;
+  const T* ru = wu + f * ldw;
+#pragma unroll 2
+  for (int k = lane * V; k < d; k += 64 * V) {
+    const Pack<T, V> g = *reinterpret_cast<const Pack<T, V>*>(rg + k);
+    const Pack<T, V> w = *reinterpret_cast<const Pack<T, V>*>(ru + k);
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      if (i < m) {
+        const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(x + i * ldx + k);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          sa[i] = fmaf(to_f32(v.v[e]), to_f32(g.v[e]), sa[i]);
+          su[i] = fmaf(to_f32(v.v[e]), to_f32(w.v[e]), su[i]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < M; ++i)
+#pragma unroll
+    for (int s = 32; s >= 1; s >>= 1) {
+      sa[i] += __shfl_xor(sa[i], s);
+      su[i] += __shfl_xor(su[i], s);
+    }
+  if (lane == 0) {
+    const float b0 = bg ? to_f32(bg[f]) : 0.f, b1 = bu ? to_f32(bu[f]) : 0.f;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      if (i < m) {
+        const float za = sa[i] + b0, zu = su[i] + b1;
+        const int64_t at = (int64_t)i * n + f;
+        h[at] = from_f32<T>(act_value<sizeof(T) == 4>(act, za) * zu);
+        if (a) { a[at] = za; u[at] = zu; }
+      }
+    }
+  }
+}
+
+// ---- launches -----------------------------------------------------------------------------------------------------
+constexpr int kCus = 256;
+constexpr int kFewRows = 8;
+
+struct Tiling { int bm, bn, splits, slices_per_split, tiles_m, tiles_n; };
+
+// columns: of the tiles (forward: 2 n).  A big tile needs two passes over the machine to pay for its tail.
+Tiling tiling(int dtype, int m, int columns, int k, int halves, bool may_split) {
+  Tiling t;
+  const int kk = kSliceBytes / (dtype == PS_DTYPE_F32 ? 4 : 2);
+  auto count = [](int a, int b) { return (a + b - 1) / b; };
+  t.bm = t.bn = 128;
+  if (dtype != PS_DTYPE_F32 && (int64_t)count(m, 256) * count(columns, 256) >= 2 * kCus) t.bm = t.bn = 256;
+  t.tiles_m = count(m, t.bm);
+  t.tiles_n = count(columns, t.bn);
+  const int slices = count(k, kk) * halves, tiles = t.tiles_m * t.tiles_n;
+  t.splits = 1;
+  if (may_split && tiles < kCus) {               // fill the machine, at least 8 slices a split
+    int s = (2 * kCus) / tiles;
+    if (s > slices / 8) s = slices / 8;
+    t.splits = s < 1 ? 1 : s;
+  }
+  t.slices_per_split = count(slices, t.splits);
+  t.splits = count(slices, t.slices_per_split);
+  return t;
+}
+
+template <typename T, bool A_ACROSS, bool B_ACROSS, bool PAIRED, typename EP>
+int launch_product(Product g, const Tiling& t, const EP& ep, hipStream_t st) {
+  g.tiles_m = t.tiles_m;
+  g.tiles_n = t.tiles_n;
+  g.splits = t.splits;
+  g.slices_per_split = t.slices_per_split;
+  const dim3 grid((unsigned)(t.tiles_m * t.tiles_n), (unsigned)t.splits);
+  const size_t lds = (size_t)2 * (t.bm + t.bn) * kSliceBytes;
+  if constexpr (sizeof(T) == 2) {
+    if (t.bm == 256) {
+      auto kernel = product_kernel<T, 256, 256, 2, 4, A_ACROSS, B_ACROSS, PAIRED, EP>;
+      if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) !=
+          hipSuccess)
+        return PS_ERR_LAUNCH;
+      kernel<<<grid, 512, lds, st>>>(g, ep);
+      return PS_OK;
+    }
+  }
+  product_kernel<T, 128, 128, 2, 2, A_ACROSS, B_ACROSS, PAIRED, EP><<<grid, 256, lds, st>>>(g, ep);
+  return PS_OK;
+}
+
+int pad8(int n) { return (n + 7) & ~7; }
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+struct BackwardPlan {
+  int ld, sum_parts, slope_rows;
+  Tiling again, dx, dw;
+  size_t da, du, sums, parts, total;
+};
+
+BackwardPlan backward_plan(const PsGatedLinearDesc& d) {
+  BackwardPlan p;
+  const size_t e = d.dtype == PS_DTYPE_F32 ? 4 : 2;
+  p.ld = pad8(d.hidden);
+  p.again = tiling(d.dtype, d.rows, 2 * p.ld, d.dim, 1, false);
+  p.dx = tiling(d.dtype, d.rows, d.dim, d.hidden, 2, true);
+  p.dw = tiling(d.dtype, d.hidden, d.dim, d.rows, 1, true);
+  p.slope_rows = 32;
+  p.sum_parts = d.dtype == PS_DTYPE_F32 ? (d.rows + p.slope_rows - 1) / p.slope_rows : p.again.tiles_m * 2;
+  size_t at = 0;
+  p.da = at; at += align256(e * d.rows * p.ld);
+  p.du = at; at += align256(e * d.rows * p.ld);
+  p.sums = at; at += align256(sizeof(float) * p.sum_parts * 2 * p.ld);
+  p.parts = at;
+  const size_t px = p.dx.splits > 1 ? sizeof(float) * p.dx.splits * (size_t)d.rows * d.dim : 0;
+  const size_t pw = p.dw.splits > 1 ? sizeof(float) * p.dw.splits * (size_t)d.hidden * d.dim : 0;
+  at += align256(px > pw ? px : pw);
+  p.total = at;
+  return p;
+}
+
+template <typename T>
+int forward_typed(const PsGatedLinearDesc& d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu,
+                  void* h, float* a, float* u, hipStream_t st) {
+  if (d.rows <= kFewRows) {
+    const unsigned grid = (unsigned)((d.hidden + 3) / 4);
+    auto run = [&](auto kernel) {
+      kernel<<<grid, 256, 0, st>>>(d.rows, d.dim, d.hidden, d.activation, (const T*)x, d.x_row_stride, (const T*)wg,
+                                   (const T*)wu, d.w_row_stride, (const T*)bg, (const T*)bu, (T*)h, a, u);
+    };
+    if (d.rows == 1) run(gated_rows_kernel<T, 1>);
+    else if (d.rows == 2) run(gated_rows_kernel<T, 2>);
+    else if (d.rows <= 4) run(gated_rows_kernel<T, 4>);
+    else run(gated_rows_kernel<T, kFewRows>);
+    return PS_OK;
+  }
+  Product g = {};
+  g.m = d.rows; g.n = d.hidden; g.k = d.dim; g.halves = 1;
+  g.a.p[0] = x; g.a.ld = d.x_row_stride;
+  g.b.p[0] = wg; g.b.p[1] = wu; g.b.ld = d.w_row_stride;
+  StoreGated ep = {h, bg, bu, a, u, d.activation};
+  return launch_product<T, false, false, true>(g, tiling(d.dtype, d.rows, 2 * d.hidden, d.dim, 1, false), ep, st);
+}
+
+template <typename T>
+int join(const Tiling& t, int64_t count, const float* parts, void* c, hipStream_t st) {
+  if (t.splits > 1)
+    join_parts_kernel<T><<<(unsigned)((count + 255) / 256), 256, 0, st>>>(count, t.splits, parts, (T*)c);
+  return PS_OK;
+}
+
+template <typename T>
+int backward_typed(const PsGatedLinearDesc& d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu,
+                   const float* a, const float* u, const void* dh, void* dx, void* dwg, void* dwu, void* dbg, void* dbu,
+                   char* ws, hipStream_t st) {
+  const BackwardPlan p = backward_plan(d);
+  T* da = (T*)(ws + p.da);
+  T* du = (T*)(ws + p.du);
+  float* sums = dbg || dbu ? (float*)(ws + p.sums) : nullptr;
+  float* parts = (float*)(ws + p.parts);
+  if constexpr (sizeof(T) == 4) {
+    const dim3 grid((unsigned)((p.ld + 255) / 256), (unsigned)p.sum_parts);
+    gated_slope_kernel<<<grid, 256, 0, st>>>(d.rows, d.hidden, p.ld, p.slope_rows, d.activation, a, u, (const float*)dh,
+                                             d.dh_row_stride, da, du, sums);
+  } else {
+    Product g = {};
+    g.m = d.rows; g.n = d.hidden; g.k = d.dim; g.halves = 1;
+    g.a.p[0] = x; g.a.ld = d.x_row_stride;
+    g.b.p[0] = wg; g.b.p[1] = wu; g.b.ld = d.w_row_stride;
+    StoreGatedGrad ep = {dh, d.dh_row_stride, bg, bu, da, du, p.ld, sums, d.activation};
+    if (int rc = launch_product<T, false, false, true>(g, p.again, ep, st)) return rc;
+  }
+  if (sums)
+    gated_bias_kernel<T><<<(unsigned)((2 * p.ld + 15) / 16), 256, 0, st>>>(p.sum_parts, d.hidden, p.ld, sums, (T*)dbg, (T*)dbu);
+  if (dx) {
+    Product g = {};
+    g.m = d.rows; g.n = d.dim; g.k = d.hidden; g.halves = 2;
+    g.a.p[0] = da; g.a.p[1] = du; g.a.ld = p.ld;
+    g.b.p[0] = wg; g.b.p[1] = wu; g.b.ld = d.w_row_stride;
+    StoreMatrix ep = {dx, p.dx.splits > 1 ? parts : nullptr};
+    if (int rc = launch_product<T, false, true, false>(g, p.dx, ep, st)) return rc;
+    join<T>(p.dx, (int64_t)d.rows * d.dim, parts, dx, st);
+  }
+  for (int half = 0; half < 2; ++half) {
+    void* dw = half ? dwu : dwg;
+    if (!dw) continue;
+    Product g = {};
+    g.m = d.hidden; g.n = d.dim; g.k = d.rows; g.halves = 1;
+    g.a.p[0] = half ? du : da; g.a.ld = p.ld;
+    g.b.p[0] = x; g.b.ld = d.x_row_stride;
+    StoreMatrix ep = {dw, p.dw.splits > 1 ? parts : nullptr};
+    if (int rc = launch_product<T, true, true, false>(g, p.dw, ep, st)) return rc;
+    join<T>(p.dw, (int64_t)d.hidden * d.dim, parts, dw, st);
+  }
+  return PS_OK;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// both operands of every product are copied in 16-byte chunks: rows start on 16 bytes and hold whole chunks
+int check(const PsGatedLinearDesc* d, const void* x, const void* wg, const void* wu) {
+  if (!d || !x || !wg || !wu || d->rows <= 0 || d->dim <= 0 || d->hidden <= 0) return PS_ERR_BAD_ARG;
+  if (d->dtype < PS_DTYPE_F32 || d->dtype > PS_DTYPE_F16 || d->activation < PS_ACT_NONE || d->activation > PS_ACT_SIGMOID)
+    return PS_ERR_UNSUPPORTED;
+  if (d->rows > (1 << 28) || d->dim > (1 << 24) || d->hidden > (1 << 24)) return PS_ERR_UNSUPPORTED;
+  const int chunk = d->dtype == PS_DTYPE_F32 ? 4 : 8;
+  if (d->dim % chunk || d->x_row_stride < d->dim || d->w_row_stride < d->dim || d->x_row_stride % chunk ||
+      d->w_row_stride % chunk || !aligned16(x) || !aligned16(wg) || !aligned16(wu))
+    return PS_ERR_BAD_ARG;
+  const int64_t tiles = ((int64_t)d->rows + 127) / 128 * ((2 * (int64_t)d->hidden + 127) / 128 + (d->dim + 127) / 128);
+  return tiles < (int64_t)1 << 31 ? PS_OK : PS_ERR_UNSUPPORTED;
+}
+
+}  // namespace
+}  // namespace ps
+
+using namespace ps;
+
+extern "C" {
+
+int ps_gated_linear_forward(const PsGatedLinearDesc* d, const void* x, const void* w_gate, const void* w_up,
+                            const void* b_gate, const void* b_up, void* h, float* gate, float* up, void* stream) {
+  if (int rc = check(d, x, w_gate, w_up)) return rc;
+  if (!h || (gate == nullptr) != (up == nullptr)) return PS_ERR_BAD_ARG;
+  hipStream_t st = (hipStream_t)stream;
+  int rc;
+  switch (d->dtype) {
+    case PS_DTYPE_F32: rc = forward_typed<float>(*d, x, w_gate, w_up, b_gate, b_up, h, gate, up, st); break;
+    case PS_DTYPE_BF16: rc = forward_typed<bf16>(*d, x, w_gate, w_up, b_gate, b_up, h, gate, up, st); break;
+    default: rc = forward_typed<f16>(*d, x, w_gate, w_up, b_gate, b_up, h, gate, up, st); break;
+  }
+  return rc ? rc : hipGetLastError() == hipSuccess ? PS_OK : PS_ERR_LAUNCH;
+}
+
+size_t ps_gated_linear_backward_workspace_bytes(const PsGatedLinearDesc* d) {
+  const void* p = reinterpret_cast<const void*>(16);
+  return check(d, p, p, p) ? 0 : backward_plan(*d).total;
+}
+
+int ps_gated_linear_backward(const PsGatedLinearDesc* d, const void* x, const void* w_gate, const void* w_up,
+                             const void* b_gate, const void* b_up, const float* gate, const float* up, const void* dh,
+                             void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  if (int rc = check(d, x, w_gate, w_up)) return rc;
+  if (!dh || !workspace || !aligned16(workspace) || d->dh_row_stride < d->hidden) return PS_ERR_BAD_ARG;
+  if (d->dtype == PS_DTYPE_F32 && (!gate || !up)) return PS_ERR_BAD_ARG;
+  if (workspace_bytes < backward_plan(*d).total) return PS_ERR_WORKSPACE;
+  hipStream_t st = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  int rc;
+  switch (d->dtype) {
+    case PS_DTYPE_F32: rc = backward_typed<float>(*d, x, w_gate, w_up, b_gate, b_up, gate, up, dh, dx, dw_gate, dw_up, db_gate, db_up, ws, st); break;
+    case PS_DTYPE_BF16: rc = backward_typed<bf16>(*d, x, w_gate, w_up, b_gate, b_up, gate, up, dh, dx, dw_gate, dw_up, db_gate, db_up, ws, st); break;
+    default: rc = backward_typed<f16>(*d, x, w_gate, w_up, b_gate, b_up, gate, up, dh, dx, dw_gate, dw_up, db_gate, db_up, ws, st); break;
+  }
+  return rc ? rc : hipGetLastError() == hipSuccess ? PS_OK : PS_ERR_LAUNCH;
+}
+
+}  // extern "C"

@@ -49,6 +49,27 @@ int ps_group_norm_backward(const PsGroupNormDesc* desc, const void* x, const voi
                            const void* beta, const float* mean, const float* rstd, void* dx, void* d_gamma,
                            void* d_beta, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Gated projection of a feed-forward block, h = act(x w_gate^T + b_gate) * (x w_up^T + b_up): x [rows][dim], weights
+ * [hidden][dim] (one row stride for both), biases [hidden] in the tensors' type, each may be NULL; h [rows][hidden]
+ * contiguous.  dim and the strides of x and of the weights are whole numbers of 16-byte chunks and the three
+ * matrices are 16-byte aligned (else PS_ERR_BAD_ARG); hidden is any number.  No projection is written to memory,
+ * except gate, up [rows][hidden] fp32 (the projections with their biases) where they are not NULL: fp32 training
+ * hands them to the backward, 16-bit types compute them again and take NULL there.
+ * Backward: every output may be NULL.  dx [rows][dim], dw [hidden][dim], db [hidden], contiguous. */
+typedef struct PsGatedLinearDesc {
+  int32_t rows, dim, hidden;
+  int32_t dtype, activation;
+  int32_t reserved; /* 0 */
+  int64_t x_row_stride, w_row_stride, dh_row_stride;
+} PsGatedLinearDesc;
+int ps_gated_linear_forward(const PsGatedLinearDesc* desc, const void* x, const void* w_gate, const void* w_up,
+                            const void* b_gate, const void* b_up, void* h, float* gate, float* up, void* stream);
+size_t ps_gated_linear_backward_workspace_bytes(const PsGatedLinearDesc* desc);
+int ps_gated_linear_backward(const PsGatedLinearDesc* desc, const void* x, const void* w_gate, const void* w_up,
+                             const void* b_gate, const void* b_up, const float* gate, const float* up, const void* dh,
+                             void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
 /* "pixelsplat_ops gfx950 | <file>:<hash> ...", as ps_build_info of pixelsplat_hip.h. */
 const char* ps_ops_build_info(void);
 

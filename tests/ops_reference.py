@@ -42,3 +42,30 @@ def within(got, want, bound, what):
     at = int(over.argmax())
     assert (over <= 0).all(), (f"{what}: element {at}: {got.flatten()[at].item():.9g} for {want.flatten()[at].item():.9g}, "
                                f"{over.flatten()[at].item():.3g} over the bound")
+
+
+def slope(name, z):
+    """act'(z), and a bound of |act''| (relu: its jump is the caller's)"""
+    if name == "none":
+        return torch.ones_like(z)
+    if name == "relu":
+        return (z > 0).to(z.dtype)
+    s = torch.sigmoid(z)
+    if name == "silu":
+        return s * (1 + z * (1 - s))
+    if name == "gelu":
+        return 0.5 * torch.erfc(-z / math.sqrt(2)) + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    return s * (1 - s)
+
+
+def gated_linear(x, wg, wu, bg, bu, activation, dh=None):
+    """h, and with dh the gradients and what their bounds need (formulas, 64 bits)"""
+    a, u = x @ wg.T, x @ wu.T
+    a = a if bg is None else a + bg
+    u = u if bu is None else u + bu
+    value = act(activation, a)
+    if dh is None:
+        return value * u
+    du, da = dh * value, dh * u * slope(activation, a)
+    return value * u, dict(x=da @ wg + du @ wu, w_gate=da.T @ x, w_up=du.T @ x, b_gate=da.sum(0), b_up=du.sum(0)), \
+        dict(a=a, u=u, value=value, da=da, du=du)

@@ -95,3 +95,54 @@ def test_group_norm_c_abi_refusals(lib):
         bad = _lib.PsGroupNormDesc(**{**good, field: value})
         assert forward(bad) == status and backward(bad) == status, field
         assert lib.ps_group_norm_workspace_bytes(C.byref(bad), 1) == 0
+
+
+def test_gated_linear_refusals(lib):
+    from pixelsplat_amd.ops import gated_linear
+    x, w, b = torch.zeros(3, 8), torch.zeros(5, 8), torch.zeros(5)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        gated_linear(x, w, w)
+    with pytest.raises(TypeError, match="int32"):
+        gated_linear(x.int(), w, w)
+    fake = lambda *s, dtype=torch.float32: _FakeGpu(torch.zeros(s, dtype=dtype))  # noqa: E731
+    with pytest.raises(RuntimeError, match="w_up is on"):
+        gated_linear(fake(3, 8), fake(5, 8), w)
+    for args in [(fake(3, 8), fake(5, 7), fake(5, 7)), (fake(3, 8), fake(5, 8), fake(6, 8)), (fake(3, 8), fake(8), fake(8))]:
+        with pytest.raises(ValueError, match="two weights"):
+            gated_linear(*args)
+    with pytest.raises(ValueError, match="w_up is"):
+        gated_linear(fake(3, 8), fake(5, 8), fake(5, 8, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="b_gate is"):
+        gated_linear(fake(3, 8), fake(5, 8), fake(5, 8), fake(4))
+    with pytest.raises(ValueError, match="activation"):
+        gated_linear(fake(3, 8), fake(5, 8), fake(5, 8), activation="tanh")
+    with pytest.raises(ValueError, match="dim is 0"):
+        gated_linear(fake(3, 0), fake(5, 0), fake(5, 0))
+
+
+def test_gated_linear_c_abi_refusals(lib):
+    from pixelsplat_amd.ops import _lib
+    good = dict(rows=6, dim=16, hidden=5, dtype=1, activation=2, reserved=0, x_row_stride=16, w_row_stride=16,
+                dh_row_stride=5)
+    p = 4096          # an address that is never followed
+    ok = _lib.PsGatedLinearDesc(**good)
+    assert lib.ps_gated_linear_backward_workspace_bytes(C.byref(ok)) > 0
+
+    def forward(d, x=p, wu=p, h=p, gate=None, up=None):
+        return lib.ps_gated_linear_forward(C.byref(d) if d else None, x, p, wu, None, None, h, gate, up, None)
+
+    def backward(d, dh=p, gate=p, ws=p, n=1 << 40):
+        return lib.ps_gated_linear_backward(C.byref(d) if d else None, p, p, p, None, None, gate, gate, dh, None, None,
+                                            None, None, None, ws, n, None)
+
+    assert forward(None) == backward(None) == forward(ok, x=None) == forward(ok, x=p + 2) == forward(ok, wu=p + 8) == -1
+    assert forward(ok, h=None) == forward(ok, gate=p) == backward(ok, dh=None) == backward(ok, ws=p + 4) == -1
+    assert backward(_lib.PsGatedLinearDesc(**{**good, "dtype": 0}), gate=None) == -1
+    assert backward(ok, n=100) == -2
+    for field, value, status in [("rows", 0, -1), ("dim", 0, -1), ("hidden", -1, -1), ("dim", 12, -1),
+                                 ("x_row_stride", 8, -1), ("x_row_stride", 20, -1), ("w_row_stride", 17, -1),
+                                 ("dtype", 3, -4), ("activation", 5, -4), ("rows", 1 << 30, -4)]:
+        bad = _lib.PsGatedLinearDesc(**{**good, field: value})
+        assert forward(bad) == status and backward(bad) == status, field
+        assert lib.ps_gated_linear_backward_workspace_bytes(C.byref(bad)) == 0
+    assert backward(_lib.PsGatedLinearDesc(**{**good, "dh_row_stride": 4})) == -1
