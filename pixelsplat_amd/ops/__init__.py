@@ -2,3 +2,5 @@
 tensors on the GPU, each with its backward pass."""
 from .group_norm import GroupNormAct, group_norm  # noqa: F401
 from .gated_linear import gated_linear  # noqa: F401
+from .relative_attention import (RelativePositionBias, relative_attention, relative_bucket_count,  # noqa: F401
+                                 relative_buckets)

@@ -30,8 +30,14 @@ class PsGatedLinearDesc(C.Structure):
         (n, C.c_int64) for n in ("x_row_stride", "w_row_stride", "dh_row_stride")]
 
 
+class PsRelativeAttentionDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "heads", "queries", "query_start", "grid_h", "grid_w", "dim", "dtype",
+                                         "buckets", "table_f32")] + [("scale", C.c_float), ("reserved", C.c_int32)] + [
+        (n, C.c_int64 * 3) for n in ("q_strides", "k_strides", "v_strides", "do_strides")] + [("mask_stride", C.c_int64)]
+
+
 _vp, _size, _i32 = C.c_void_p, C.c_size_t, C.c_int32
-_pn, _pg = C.POINTER(PsGroupNormDesc), C.POINTER(PsGatedLinearDesc)
+_pn, _pg, _pa = (C.POINTER(t) for t in (PsGroupNormDesc, PsGatedLinearDesc, PsRelativeAttentionDesc))
 # every symbol pixelsplat_ops.h declares: (result, arguments)
 SIGNATURES = {
     "ps_group_norm_workspace_bytes": (_size, [_pn, _i32]),
@@ -40,6 +46,9 @@ SIGNATURES = {
     "ps_gated_linear_forward": (C.c_int, [_pg] + [_vp] * 9),
     "ps_gated_linear_backward_workspace_bytes": (_size, [_pg]),
     "ps_gated_linear_backward": (C.c_int, [_pg] + [_vp] * 14 + [_size, _vp]),
+    "ps_relative_attention_workspace_bytes": (_size, [_pa, _i32]),
+    "ps_relative_attention_forward": (C.c_int, [_pa] + [_vp] * 11 + [_size, _vp]),
+    "ps_relative_attention_backward": (C.c_int, [_pa] + [_vp] * 14 + [_size, _vp]),
     "ps_ops_build_info": (C.c_char_p, []),
 }
 

@@ -1,0 +1,933 @@
+// Attention over a token grid with a learned relative position bias,
+//   s = scale q.k + table[bucket[key - query]][head];  p = softmax(s) over the keys that are there;  o = p v,
+// and its backward pass
+//   dp = do.v;  ds = p (dp - do.o);  dq = scale ds k;  dk = scale ds^T q;  dv = p^T do;
+//   d_table[b][head] = sum of ds over the batch and the pairs whose offset has bucket b.
+//
+// Tokens of a gh x gw grid are numbered by rows; code(t) = row (2 gw - 1) + column, so that the flattened (row, column)
+// offset of a pair is code(key) - code(query) + origin.  A first small kernel spreads the table over the offsets, per
+// head; a block then needs, for a tile of keys, one contiguous window of that, which it copies to LDS with the keys.
+//
+// Layout of the work.  A wave owns 32 queries (forward, dq) or 32 keys (dk, dv) as the COLUMNS of its products -- their
+// operands stay in registers for the whole pass -- and streams the other side through LDS, double buffered, copied
+// straight from global memory.  With columns in lanes, the 32 x 32 result of the first product has its rows in
+// registers, which is what the second product contracts over: probabilities and ds go from the result registers into
+// operand registers with no shuffle and no LDS (the order of the contraction index follows the registers', and the other
+// operand is read in that order).  Softmax statistics are one value a lane.
+//
+// Logits are kept times log2(e): one exp2 an element.  Sums, statistics and do.o are fp32.  p and ds are rounded to the
+// tensors' type as operands of their second product, the sums of p are not.  In 16-bit training the forward keeps o in
+// fp32 too: do.o of the rounded o would put its rounding into every ds of the row.  A row's maximum and the inverse of
+// its sum are kept apart: their sum as a logarithm would lose the second where all biases of a row are at the lowest value.
+//
+// d_table without atomics on memory, in a fixed order: in the dq pass each wave adds its ds into a ring of its own in
+// LDS, indexed by code(key) + const - code(query); the 32 queries of a half wave have 32 different offsets to one key,
+// and the halves add one after the other.  What lies behind the next tile's first code is final and leaves the ring
+// for the wave's row in memory; two small kernels add the rows of all waves by offset and the offsets by bucket.
+//
+// Bound by the matrix instructions in fp32, by the vector instructions of the softmax in 16 bits, by the keys' and
+// values' bytes for a few queries, which split the keys over blocks and join their partial results.
+#include "mfma_tile.h"
+#include "pixelsplat_ops.h"
+
+namespace ps {
+namespace {
+
+__device__ const uint4 kZeros[1] = {{0, 0, 0, 0}};
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kInf = __builtin_inff();
+
+struct Strides { int64_t b, h, t; };
+
+struct Args {
+  const void *q, *k, *v;
+  Strides sq, sk, sv;
+  const uint8_t* mask;            // [batch][nk] or NULL
+  int64_t mask_b;
+  const float* bias;              // [heads][offsets], times log2(e)
+  int batch, heads, nq, nk, dim, gw, origin, offsets, q_start, nq_pad;
+  float scale;
+  int window;                     // floats of a window in LDS, a multiple of 64
+  int col_tiles, splits, tiles_per_split;
+  // forward
+  void* out;                      // [batch][nq][heads][dim]
+  float* o32;                     // the same in fp32 or NULL
+  float* stats;                   // [2][batch heads][nq_pad] or NULL: maximum (log2; +inf: no keys), 1 / sum (0: no keys)
+  float *part_o, *part_ml;        // [splits][batch heads nq][dim], [..][2]
+  // backward
+  const void* dout;
+  Strides sdo;
+  const float* o_kept;            // fp32 o
+  float* delta;                   // [batch heads][nq_pad]: do.o / sum
+  void *dq, *dk, *dv;
+  float* ring_rows;               // [batch heads][nq_pad / 32][ring_pitch]
+  int ring, ring_pitch;
+};
+
+__device__ __forceinline__ int code_of(int t, int gw) { return t + (int)((unsigned)t / (unsigned)gw) * (gw - 1); }
+
+template <typename T> constexpr int kRows = sizeof(T) == 2 ? 64 : 32;   // rows of a streamed tile
+
+// ---- streamed tiles: [rows][PITCH bytes], 16-byte chunk c of row r at c ^ swizzle(r) -----------------------------
+// Both reads are free of bank conflicts: 16 rows at one chunk (the swizzle takes all values over 16 rows that do not
+// differ in their bank already), and 4 rows at four neighbouring chunks (its high bits come from r & 3).
+template <int PITCH>
+__device__ __forceinline__ int swizzle(int r) {
+  if (PITCH % 256 == 0) return ((r & 3) << 2) | ((r >> 2) & 3);
+  if (PITCH % 256 == 128) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+  return (r >> 2) & 3;
+}
+
+template <typename T, int PITCH>
+__device__ __forceinline__ Frag<T> along(const char* tile, int row, int chunk) {
+  return *reinterpret_cast<const Frag<T>*>(tile + row * PITCH + ((chunk ^ swizzle<PITCH>(row)) << 4));
+}
+
+// columns d0 .. d0 + 31 of the rows that registers kVec * s .. of a result hold
+template <typename T, int PITCH>
+__device__ __forceinline__ Frag<T> across(const char* tile, int row0, int s, int d0, int lane) {
+  const int hi = lane >> 5;
+  if constexpr (sizeof(T) == 2) {
+    typedef __attribute__((address_space(3))) shortx4 lds_shortx4;
+    const int i = lane & 15, kr = i >> 2, col = (lane & 16) + (i & 3) * 4;
+    const int r0 = row0 + 16 * s + 4 * hi + kr, r1 = r0 + 8, chunk = (d0 + col) >> 3, in = (col & 4) * 2;
+    const shortx4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_shortx4*)(tile + r0 * PITCH + ((chunk ^ swizzle<PITCH>(r0)) << 4) + in));
+    const shortx4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_shortx4*)(tile + r1 * PITCH + ((chunk ^ swizzle<PITCH>(r1)) << 4) + in));
+    return __builtin_bit_cast(Frag<T>, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+  } else {
+    const int col = d0 + (lane & 31);
+    Frag<T> v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = row0 + 8 * s + 4 * hi + j;
+      v[j] = *reinterpret_cast<const float*>(tile + r * PITCH + (((col >> 2) ^ swizzle<PITCH>(r)) << 4) + (col & 3) * 4);
+    }
+    return v;
+  }
+}
+
+// registers kVec * s .. of a result as an operand
+template <typename T>
+__device__ __forceinline__ Frag<T> as_operand(const floatx16& r, int s) {
+  Frag<T> f;
+#pragma unroll
+  for (int e = 0; e < kVec<T>; ++e) f[e] = from_f32<T>(r[s * kVec<T> + e]);
+  return f;
+}
+
+// rows `bits` of the tile at `base` (row stride `stride` elements); rows that are not there become zeros
+template <typename T, int PITCH, int ROWS, int WAVES>
+__device__ __forceinline__ void copy_tile(const T* base, int64_t stride, int dim, uint64_t bits, char* tile, int wave,
+                                          int lane) {
+  constexpr int kChunks = PITCH / 16, kPieces = ROWS * PITCH / 1024;
+#pragma unroll
+  for (int j = 0; j < kPieces / WAVES; ++j) {
+    const int pos = (j * WAVES + wave) * 64 + lane, row = pos / kChunks;
+    const int d = ((pos % kChunks) ^ swizzle<PITCH>(row)) * kVec<T>;
+    const bool on = ((bits >> row) & 1) && d < dim;
+    copy_to_lds(on ? (const void*)(base + (row * (int)stride + d)) : (const void*)kZeros, tile + (j * WAVES + wave) * 1024);
+  }
+}
+
+// offsets first .. first + window of the head's bias
+template <int WAVES>
+__device__ __forceinline__ void copy_window(const float* bias, int offsets, int first, int window, float* lds, int wave,
+                                            int lane) {
+  for (int i = wave * 64; i < window; i += WAVES * 64)
+    __builtin_amdgcn_global_load_lds(
+        (const __attribute__((address_space(1))) void*)(bias + min(max(first + i + lane, 0), offsets - 1)),
+        (__attribute__((address_space(3))) void*)(lds + i), 4, 0, 0);
+}
+
+// a lane's column operand: 16-byte chunks 2 s + hi of its row
+template <typename T, int DP>
+__device__ __forceinline__ void load_columns(Frag<T> (&f)[DP / kFragK<T>], const T* row, bool on, int dim, int hi) {
+#pragma unroll
+  for (int s = 0; s < DP / kFragK<T>; ++s) {
+    const int d = (2 * s + hi) * kVec<T>;
+    f[s] = *reinterpret_cast<const Frag<T>*>(on && d < dim ? (const void*)(row + d) : (const void*)kZeros);
+  }
+}
+
+// the columns' result [DP x 32], transposed into rows of `out` (dim elements each), times `by`
+template <typename T, int DP>
+__device__ __forceinline__ void store_columns(const floatx16 (&acc)[DP / 32], float by, T* row, int dim, int hi) {
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int d = t * 32 + 8 * a + 4 * hi;
+      if (d < dim) {                                   // dim is a multiple of 4
+        Pack<T, 4> v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v.v[j] = from_f32<T>(acc[t][4 * a + j] * by);
+        *reinterpret_cast<Pack<T, 4>*>(row + d) = v;
+      }
+    }
+}
+
+template <typename T, int DP, int WAVES>
+struct Lds {                                            // bytes
+  static constexpr int kTile = kRows<T> * DP * (int)sizeof(T);
+  static constexpr int kRowData = 64 * 4;               // one word a row
+  static constexpr int kWindow = 2 * kTile + 4 * kRowData;
+  // [2][first tile | second tile | codes | row data 1 | 2 | 3 | window]
+  __host__ __device__ static int buffer(int window) { return kWindow + window * 4; }
+};
+
+// whether the lane's row of a tile is there
+__device__ __forceinline__ bool row_there(int first, int count, int rows, const uint8_t* mask, int lane) {
+  const int i = first + lane;
+  return lane < rows && i < count && (mask == nullptr || mask[i] != 0);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(256) spread_table_kernel(int heads, int offsets, int buckets, const int32_t* __restrict__ map,
+                                                           const void* __restrict__ table, int table_f32,
+                                                           float* __restrict__ bias) {
+  const int o = blockIdx.x * 256 + threadIdx.x;
+  if (o >= offsets) return;
+  const int bucket = map[o];
+  const bool on = bucket >= 0 && bucket < buckets;
+  for (int h = blockIdx.y; h < heads; h += gridDim.y) {
+    const float v = on ? load_param<T>(table, table_f32, (int64_t)bucket * heads + h) : 0.f;
+    // a bias at the types' lowest value stays finite after the factor: a row of nothing else is uniform, not empty
+    float b = v * kLog2e;
+    if (b < -3e38f && v != -kInf) b = -3e38f;
+    if (b > 3e38f && v != kInf) b = 3e38f;
+    bias[(int64_t)h * offsets + o] = b;
+  }
+}
+
+template <typename T, int DP, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64, DP == 128 && (sizeof(T) == 4 || WAVES == 1) ? 1 : 2) attention_forward_kernel(Args p) {
+  constexpr int PITCH = DP * sizeof(T), ROWS = kRows<T>, SUBS = ROWS / 32, KF = DP / kFragK<T>, PF = 32 / kFragK<T>;
+  typedef Lds<T, DP, WAVES> L;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, hi = lane >> 5;
+  const int tile = blockIdx.x % p.col_tiles, bh = blockIdx.x / p.col_tiles, split = blockIdx.y;
+  const int b = bh / p.heads, h = bh % p.heads;
+  const int first = tile * WAVES * 32, last = min(first + WAVES * 32, p.nq) - 1;
+  const int qi = first + wave * 32 + (lane & 31);
+  const bool q_on = qi < p.nq;
+  const int code_last = code_of(p.q_start + max(last, 0), p.gw);
+  const int q_off = code_last - code_of(p.q_start + min(qi, max(last, 0)), p.gw);
+
+  Frag<T> qf[KF];
+  load_columns<T, DP>(qf, (const T*)p.q + b * p.sq.b + h * p.sq.h + qi * p.sq.t, q_on, p.dim, hi);
+  const T* kb = (const T*)p.k + b * p.sk.b + h * p.sk.h;
+  const T* vb = (const T*)p.v + b * p.sv.b + h * p.sv.h;
+  const uint8_t* mask = p.mask ? p.mask + b * p.mask_b : nullptr;
+  const float* bias = p.bias + (int64_t)h * p.offsets;
+  const int bytes = L::buffer(p.window);
+
+  floatx16 o[DP / 32];
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t) o[t] = zero16();
+  float m = -kInf, l = 0.f;
+
+  const int tiles = (p.nk + ROWS - 1) / ROWS;
+  const int t0 = split * p.tiles_per_split, t1 = min(t0 + p.tiles_per_split, tiles);
+  uint64_t bits = 0, next_bits = 0;
+  bool there = row_there(t0 * ROWS, p.nk, ROWS, mask, lane);
+  auto load = [&](int kt, int buf) {
+    char* at = lds + buf * bytes;
+    const int k0 = kt * ROWS;
+    next_bits = __ballot(there);                       // read a tile ahead
+    there = row_there(k0 + ROWS, p.nk, ROWS, mask, lane);
+    copy_tile<T, PITCH, ROWS, WAVES>(kb + k0 * p.sk.t, p.sk.t, p.dim, next_bits, at, wave, lane);
+    copy_tile<T, PITCH, ROWS, WAVES>(vb + k0 * p.sv.t, p.sv.t, p.dim, next_bits, at + L::kTile, wave, lane);
+    int* codes = reinterpret_cast<int*>(at + 2 * L::kTile);
+    const int c0 = code_of(k0, p.gw);
+    if ((int)threadIdx.x < ROWS) codes[threadIdx.x] = code_of(min(k0 + (int)threadIdx.x, p.nk - 1), p.gw) - c0;
+    copy_window<WAVES>(bias, p.offsets, c0 - code_last + p.origin, p.window,
+                       reinterpret_cast<float*>(at + L::kWindow), wave, lane);
+  };
+  if (t0 < t1) load(t0, 0);
+  __syncthreads();
+  for (int kt = t0; kt < t1; ++kt) {
+    const int buf = (kt - t0) & 1;
+    bits = next_bits;
+    if (kt + 1 < t1) load(kt + 1, buf ^ 1);
+    const char* tk = lds + buf * bytes;
+    const char* tv = tk + L::kTile;
+    const int* codes = reinterpret_cast<const int*>(tk + 2 * L::kTile);
+    const float* window = reinterpret_cast<const float*>(tk + L::kWindow) + q_off;
+
+    floatx16 s[SUBS];
+    float top = -kInf;
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u) {
+      s[u] = zero16();
+#pragma unroll
+      for (int f = 0; f < KF; ++f)
+        s[u] = mfma(along<T, PITCH>(tk, u * 32 + (lane & 31), 2 * f + hi), qf[f], s[u]);
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const int4 c = *reinterpret_cast<const int4*>(codes + u * 32 + 8 * a + 4 * hi);
+        s[u][4 * a + 0] = fmaf(s[u][4 * a + 0], p.scale, window[c.x]);
+        s[u][4 * a + 1] = fmaf(s[u][4 * a + 1], p.scale, window[c.y]);
+        s[u][4 * a + 2] = fmaf(s[u][4 * a + 2], p.scale, window[c.z]);
+        s[u][4 * a + 3] = fmaf(s[u][4 * a + 3], p.scale, window[c.w]);
+      }
+    }
+    if (bits != (ROWS == 64 ? ~0ull : 0xffffffffull)) {
+#pragma unroll
+      for (int u = 0; u < SUBS; ++u) {
+        const uint32_t mine = (uint32_t)(bits >> (32 * u)) >> (4 * hi);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!((mine >> (8 * (r >> 2) + (r & 3))) & 1)) s[u][r] = -kInf;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+    top = fmaxf(top, __shfl_xor(top, 32));
+    if (__any(top > m)) {                              // a new maximum: what there is shrinks
+      const float nm = fmaxf(m, top);
+      const float by = __builtin_amdgcn_exp2f(m - (nm == -kInf ? 0.f : nm));
+      m = nm;
+      l *= by;
+#pragma unroll
+      for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[t][r] *= by;
+    }
+    const float base = m == -kInf ? 0.f : m;           // nothing yet: exp2(-inf) = 0
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[u][r] = __builtin_amdgcn_exp2f(s[u][r] - base);
+        l += s[u][r];
+      }
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u)
+#pragma unroll
+      for (int f = 0; f < PF; ++f) {
+        const Frag<T> pf = as_operand<T>(s[u], f);
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t) o[t] = mfma(across<T, PITCH>(tv, u * 32, f, t * 32, lane), pf, o[t]);
+      }
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32);
+  if (p.splits > 1) {
+    if (!q_on) return;
+    const int64_t row = ((int64_t)split * p.batch * p.heads + bh) * p.nq + qi;
+    if (hi == 0) {
+      p.part_ml[row * 2] = m;
+      p.part_ml[row * 2 + 1] = l;
+    }
+    store_columns<float, DP>(o, 1.f, p.part_o + row * p.dim, p.dim, hi);
+    return;
+  }
+  const float by = q_on && l != 0.f ? 1.f / l : 0.f;   // a row without keys is zero
+  if (p.stats && hi == 0 && qi < p.nq_pad) {
+    const int64_t at = (int64_t)bh * p.nq_pad + qi;
+    p.stats[at] = q_on && l != 0.f ? m : kInf;
+    p.stats[(int64_t)p.batch * p.heads * p.nq_pad + at] = by;
+  }
+  if (!q_on) return;
+  const int64_t row = (((int64_t)b * p.nq + qi) * p.heads + h) * p.dim;
+  store_columns<T, DP>(o, by, (T*)p.out + row, p.dim, hi);
+  if (p.o32) store_columns<float, DP>(o, by, p.o32 + row, p.dim, hi);
+}
+
+// the splits of a row, joined: a thread takes 4 columns
+template <typename T>
+__global__ void __launch_bounds__(256) join_splits_kernel(Args p) {
+  const int per = p.dim / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)p.batch * p.heads * p.nq_pad;
+  const int64_t at = i / per;
+  const int d = (int)(i % per) * 4;
+  if (at >= rows) return;
+  const int bh = (int)(at / p.nq_pad), qi = (int)(at % p.nq_pad);
+  if (qi >= p.nq) {
+    if (p.stats && d == 0) {
+      p.stats[at] = kInf;
+      p.stats[rows + at] = 0.f;
+    }
+    return;
+  }
+  const int64_t all = (int64_t)p.batch * p.heads * p.nq, row = (int64_t)bh * p.nq + qi;
+  float m = -kInf;
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[(s * all + row) * 2]);
+  const float base = m == -kInf ? 0.f : m;
+  float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.splits; ++s) {
+    const float by = __builtin_amdgcn_exp2f(p.part_ml[(s * all + row) * 2] - base);
+    l = fmaf(p.part_ml[(s * all + row) * 2 + 1], by, l);
+    const float4 v = *reinterpret_cast<const float4*>(p.part_o + (s * all + row) * p.dim + d);
+    o[0] = fmaf(v.x, by, o[0]);
+    o[1] = fmaf(v.y, by, o[1]);
+    o[2] = fmaf(v.z, by, o[2]);
+    o[3] = fmaf(v.w, by, o[3]);
+  }
+  const float by = l == 0.f ? 0.f : 1.f / l;
+  const int64_t to = (((int64_t)(bh / p.heads) * p.nq + qi) * p.heads + bh % p.heads) * p.dim + d;
+  Pack<T, 4> v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v.v[j] = from_f32<T>(o[j] * by);
+    if (p.o32) p.o32[to + j] = o[j] * by;
+  }
+  *reinterpret_cast<Pack<T, 4>*>((T*)p.out + to) = v;
+  if (p.stats && d == 0) {
+    p.stats[at] = l != 0.f ? m : kInf;
+    p.stats[rows + at] = by;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// dq, do.o and the rings of d_table.  Columns are queries, rows are keys, as in the forward.
+template <typename T, int DP, int WAVES, bool RING>
+__global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || (RING && DP == 128) ? 1 : 2) attention_dq_kernel(Args p) {
+  constexpr int PITCH = DP * sizeof(T), ROWS = kRows<T>, SUBS = ROWS / 32, KF = DP / kFragK<T>, PF = 32 / kFragK<T>;
+  typedef Lds<T, DP, WAVES> L;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, hi = lane >> 5;
+  const int tile = blockIdx.x % p.col_tiles, bh = blockIdx.x / p.col_tiles;
+  const int b = bh / p.heads, h = bh % p.heads;
+  const int first = tile * WAVES * 32, last = max(min(first + WAVES * 32, p.nq) - 1, 0);
+  const int qi = first + wave * 32 + (lane & 31);
+  const bool q_on = qi < p.nq;
+  const int code_last = code_of(p.q_start + last, p.gw);
+  const int code_mine = code_of(p.q_start + min(qi, last), p.gw);
+  const int q_off = code_last - code_mine;
+  const int bytes = L::buffer(p.window);
+
+  Frag<T> qf[KF], df[KF];
+  load_columns<T, DP>(qf, (const T*)p.q + b * p.sq.b + h * p.sq.h + qi * p.sq.t, q_on, p.dim, hi);
+  load_columns<T, DP>(df, (const T*)p.dout + b * p.sdo.b + h * p.sdo.h + qi * p.sdo.t, q_on, p.dim, hi);
+  float delta = 0.f;
+  if (q_on) {
+    const float* o = p.o_kept + (((int64_t)b * p.nq + qi) * p.heads + h) * p.dim;
+#pragma unroll
+    for (int f = 0; f < KF; ++f)
+#pragma unroll
+      for (int e = 0; e < kVec<T>; ++e) {
+        const int d = (2 * f + hi) * kVec<T> + e;
+        if (d < p.dim) delta = fmaf(to_f32(df[f][e]), o[d], delta);
+      }
+  }
+  delta += __shfl_xor(delta, 32);
+  float m = kInf, inv = 0.f;
+  if (qi < p.nq_pad) {
+    const int64_t at = (int64_t)bh * p.nq_pad + qi;
+    m = p.stats[at];
+    inv = p.stats[(int64_t)p.batch * p.heads * p.nq_pad + at];
+    delta *= inv;
+    if (hi == 0) p.delta[at] = delta;
+  }
+
+  // the wave's ring: entry u of its row is the offset u - ring_base of the head
+  float* ring = reinterpret_cast<float*>(lds + 2 * bytes) + wave * p.ring;
+  const int wave_first = min(first + wave * 32, last), wave_last = min(first + wave * 32 + 31, last);
+  const int wave_code = code_of(p.q_start + wave_last, p.gw);
+  const int ring_off = wave_code - code_of(p.q_start + min(qi, wave_last), p.gw);
+  const int q_span = wave_code - code_of(p.q_start + wave_first, p.gw);
+  const bool wave_on = first + wave * 32 < p.nq;
+  float* ring_row = nullptr;
+  if (RING) {
+    ring_row = p.ring_rows + ((int64_t)bh * (p.nq_pad / 32) + (first / 32 + wave)) * p.ring_pitch;
+    for (int i = lane; i < p.ring; i += 64) ring[i] = 0.f;
+  }
+
+  const T* kb = (const T*)p.k + b * p.sk.b + h * p.sk.h;
+  const T* vb = (const T*)p.v + b * p.sv.b + h * p.sv.h;
+  const uint8_t* mask = p.mask ? p.mask + b * p.mask_b : nullptr;
+  const float* bias = p.bias + (int64_t)h * p.offsets;
+  floatx16 dq[DP / 32];
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t) dq[t] = zero16();
+
+  const int tiles = (p.nk + ROWS - 1) / ROWS;
+  uint64_t bits = 0, next_bits = 0;
+  bool there = row_there(0, p.nk, ROWS, mask, lane);
+  auto load = [&](int kt, int buf) {
+    char* at = lds + buf * bytes;
+    const int k0 = kt * ROWS;
+    next_bits = __ballot(there);                       // read a tile ahead
+    there = row_there(k0 + ROWS, p.nk, ROWS, mask, lane);
+    copy_tile<T, PITCH, ROWS, WAVES>(kb + k0 * p.sk.t, p.sk.t, p.dim, next_bits, at, wave, lane);
+    copy_tile<T, PITCH, ROWS, WAVES>(vb + k0 * p.sv.t, p.sv.t, p.dim, next_bits, at + L::kTile, wave, lane);
+    int* codes = reinterpret_cast<int*>(at + 2 * L::kTile);
+    const int c0 = code_of(k0, p.gw);
+    if ((int)threadIdx.x < ROWS) codes[threadIdx.x] = code_of(min(k0 + (int)threadIdx.x, p.nk - 1), p.gw) - c0;
+    copy_window<WAVES>(bias, p.offsets, c0 - code_last + p.origin, p.window,
+                       reinterpret_cast<float*>(at + L::kWindow), wave, lane);
+  };
+  load(0, 0);
+  __syncthreads();
+  for (int kt = 0; kt < tiles; ++kt) {
+    const int buf = kt & 1;
+    bits = next_bits;
+    if (kt + 1 < tiles) load(kt + 1, buf ^ 1);
+    const char* tk = lds + buf * bytes;
+    const char* tv = tk + L::kTile;
+    const int* codes = reinterpret_cast<const int*>(tk + 2 * L::kTile);
+    const float* window = reinterpret_cast<const float*>(tk + L::kWindow) + q_off;
+    const int c0 = code_of(kt * ROWS, p.gw);
+    const bool whole = bits == (ROWS == 64 ? ~0ull : 0xffffffffull);
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u) {
+      floatx16 s = zero16(), ds = zero16();
+#pragma unroll
+      for (int f = 0; f < KF; ++f) {
+        s = mfma(along<T, PITCH>(tk, u * 32 + (lane & 31), 2 * f + hi), qf[f], s);
+        ds = mfma(along<T, PITCH>(tv, u * 32 + (lane & 31), 2 * f + hi), df[f], ds);
+      }
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const int4 c = *reinterpret_cast<const int4*>(codes + u * 32 + 8 * a + 4 * hi);
+        const int cs[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = 4 * a + j;
+          ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale, window[cs[j]]) - m) * fmaf(ds[r], inv, -delta);
+        }
+      }
+      if (!whole) {
+        const uint32_t mine = (uint32_t)(bits >> (32 * u)) >> (4 * hi);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!((mine >> (8 * (r >> 2) + (r & 3))) & 1)) ds[r] = 0.f;
+      }
+      if (RING && wave_on) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (hi == half) {
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+              const int4 c = *reinterpret_cast<const int4*>(codes + u * 32 + 8 * a + 4 * hi);
+              const int cs[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                __hip_atomic_fetch_add(&ring[(c0 + cs[j] + ring_off) & (p.ring - 1)], ds[4 * a + j], __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_WORKGROUP);
+            }
+          }
+          __builtin_amdgcn_wave_barrier();
+        }
+      }
+#pragma unroll
+      for (int f = 0; f < PF; ++f) {
+        const Frag<T> sf = as_operand<T>(ds, f);
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t) dq[t] = mfma(across<T, PITCH>(tk, u * 32, f, t * 32, lane), sf, dq[t]);
+      }
+    }
+    if (RING && wave_on) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const int end = kt + 1 < tiles ? code_of((kt + 1) * ROWS, p.gw) : code_of(p.nk - 1, p.gw) + q_span + 1;
+      for (int i = c0 + lane; i < end; i += 64) {
+        ring_row[i] = ring[i & (p.ring - 1)];
+        ring[i & (p.ring - 1)] = 0.f;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    __syncthreads();
+  }
+  if (q_on && p.dq)
+    store_columns<T, DP>(dq, p.scale * (1.f / kLog2e), (T*)p.dq + (((int64_t)b * p.nq + qi) * p.heads + h) * p.dim, p.dim, hi);
+}
+
+// dk, dv.  Columns are keys, rows are queries.
+template <typename T, int DP, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || DP == 128 ? 1 : 2) attention_dkv_kernel(Args p) {
+  constexpr int PITCH = DP * sizeof(T), ROWS = kRows<T>, SUBS = ROWS / 32, KF = DP / kFragK<T>, PF = 32 / kFragK<T>;
+  typedef Lds<T, DP, WAVES> L;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, hi = lane >> 5;
+  const int tile = blockIdx.x % p.col_tiles, bh = blockIdx.x / p.col_tiles;
+  const int b = bh / p.heads, h = bh % p.heads;
+  const int first = tile * WAVES * 32, last = min(first + WAVES * 32, p.nk) - 1;
+  const int ki = first + wave * 32 + (lane & 31);
+  const bool in = ki < p.nk;
+  const bool k_on = in && (p.mask == nullptr || p.mask[b * p.mask_b + ki] != 0);
+  const int code_first = code_of(first, p.gw);
+  const int k_off = code_of(min(ki, last), p.gw) - code_first;
+  const int bytes = L::buffer(p.window);
+
+  Frag<T> kf[KF], vf[KF];
+  load_columns<T, DP>(kf, (const T*)p.k + b * p.sk.b + h * p.sk.h + ki * p.sk.t, k_on, p.dim, hi);
+  load_columns<T, DP>(vf, (const T*)p.v + b * p.sv.b + h * p.sv.h + ki * p.sv.t, k_on, p.dim, hi);
+  const T* qb = (const T*)p.q + b * p.sq.b + h * p.sq.h;
+  const T* db = (const T*)p.dout + b * p.sdo.b + h * p.sdo.h;
+  const float* bias = p.bias + (int64_t)h * p.offsets;
+  const float* stat_rows[3] = {p.stats + (int64_t)bh * p.nq_pad, p.stats + ((int64_t)p.batch * p.heads + bh) * p.nq_pad,
+                               p.delta + (int64_t)bh * p.nq_pad};
+
+  floatx16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t) dk[t] = dv[t] = zero16();
+
+  const int tiles = (p.nq + ROWS - 1) / ROWS;
+  auto load = [&](int qt, int buf) {
+    char* at = lds + buf * bytes;
+    const int q0 = qt * ROWS, end = min(q0 + ROWS, p.nq) - 1;
+    const uint64_t bits = __ballot(row_there(q0, p.nq, ROWS, nullptr, lane));
+    copy_tile<T, PITCH, ROWS, WAVES>(qb + q0 * p.sq.t, p.sq.t, p.dim, bits, at, wave, lane);
+    copy_tile<T, PITCH, ROWS, WAVES>(db + q0 * p.sdo.t, p.sdo.t, p.dim, bits, at + L::kTile, wave, lane);
+    // codes count down from the tile's last query, whose window entry is the first
+    int* codes = reinterpret_cast<int*>(at + 2 * L::kTile);
+    float* rows = reinterpret_cast<float*>(at + 2 * L::kTile + L::kRowData);
+    const int c1 = code_of(p.q_start + end, p.gw);
+    if ((int)threadIdx.x < ROWS)
+      codes[threadIdx.x] = c1 - code_of(p.q_start + min(q0 + (int)threadIdx.x, end), p.gw);
+    for (int i = wave; i < 3; i += WAVES)                          // nq_pad holds whole tiles
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void*)(stat_rows[i] + q0 + min(lane, ROWS - 1)),
+          (__attribute__((address_space(3))) void*)(rows + 64 * i), 4, 0, 0);
+    copy_window<WAVES>(bias, p.offsets, code_first - c1 + p.origin, p.window,
+                       reinterpret_cast<float*>(at + L::kWindow), wave, lane);
+  };
+  load(0, 0);
+  __syncthreads();
+  for (int qt = 0; qt < tiles; ++qt) {
+    const int buf = qt & 1;
+    if (qt + 1 < tiles) load(qt + 1, buf ^ 1);
+    const char* tq = lds + buf * bytes;
+    const char* td = tq + L::kTile;
+    const int* codes = reinterpret_cast<const int*>(tq + 2 * L::kTile);
+    const float* rows = reinterpret_cast<const float*>(tq + 2 * L::kTile + L::kRowData);
+    const float* window = reinterpret_cast<const float*>(tq + L::kWindow) + k_off;
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u) {
+      floatx16 s = zero16(), ds = zero16();
+#pragma unroll
+      for (int f = 0; f < KF; ++f) {
+        s = mfma(along<T, PITCH>(tq, u * 32 + (lane & 31), 2 * f + hi), kf[f], s);
+        ds = mfma(along<T, PITCH>(td, u * 32 + (lane & 31), 2 * f + hi), vf[f], ds);
+      }
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const int4 c = *reinterpret_cast<const int4*>(codes + u * 32 + 8 * a + 4 * hi);
+        const float4 e = *reinterpret_cast<const float4*>(rows + u * 32 + 8 * a + 4 * hi);
+        const float4 w = *reinterpret_cast<const float4*>(rows + 64 + u * 32 + 8 * a + 4 * hi);
+        const float4 g = *reinterpret_cast<const float4*>(rows + 128 + u * 32 + 8 * a + 4 * hi);
+        const int cs[4] = {c.x, c.y, c.z, c.w};
+        const float es[4] = {e.x, e.y, e.z, e.w}, ws[4] = {w.x, w.y, w.z, w.w}, gs[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = 4 * a + j;
+          const float pr = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale, window[cs[j]]) - es[j]);
+          s[r] = pr * ws[j];
+          ds[r] = pr * fmaf(ds[r], ws[j], -gs[j]);
+        }
+      }
+#pragma unroll
+      for (int f = 0; f < PF; ++f) {
+        const Frag<T> pf = as_operand<T>(s, f), sf = as_operand<T>(ds, f);
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t) {
+          dv[t] = mfma(across<T, PITCH>(td, u * 32, f, t * 32, lane), pf, dv[t]);
+          dk[t] = mfma(across<T, PITCH>(tq, u * 32, f, t * 32, lane), sf, dk[t]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (in) {
+    const int64_t row = (((int64_t)b * p.nk + ki) * p.heads + h) * p.dim;
+    if (!k_on) {                                        // a key that is not there: its column held what no row saw
+#pragma unroll
+      for (int t = 0; t < DP / 32; ++t) dk[t] = dv[t] = zero16();
+    }
+    if (p.dk) store_columns<T, DP>(dk, p.scale * (1.f / kLog2e), (T*)p.dk + row, p.dim, hi);
+    if (p.dv) store_columns<T, DP>(dv, 1.f, (T*)p.dv + row, p.dim, hi);
+  }
+}
+
+// d_offsets[head][o] = sum of the rings' rows: 64 offsets a block, 4 threads an offset take every 4th row
+__global__ void __launch_bounds__(256) join_rings_kernel(Args p, double* __restrict__ d_offsets) {
+  __shared__ double lds[4][64];
+  const int o = blockIdx.x * 64 + (threadIdx.x & 63), h = blockIdx.y, part = threadIdx.x >> 6;
+  const int waves = (p.nq + 31) / 32, code_end = code_of(p.nk - 1, p.gw);
+  double t = 0;
+  if (o < p.offsets) {
+    for (int i = part; i < p.batch * waves; i += 4) {
+      const int b = i / waves, w = i % waves;
+      const int first = w * 32, last = min(first + 31, p.nq - 1);
+      const int c1 = code_of(p.q_start + last, p.gw), span = c1 - code_of(p.q_start + first, p.gw);
+      const int u = o - p.origin + c1;
+      if (u >= 0 && u <= code_end + span)
+        t += p.ring_rows[((int64_t)(b * p.heads + h) * (p.nq_pad / 32) + w) * p.ring_pitch + u];
+    }
+  }
+  lds[part][threadIdx.x & 63] = t;
+  __syncthreads();
+  if (part == 0 && o < p.offsets)
+    d_offsets[(int64_t)h * p.offsets + o] = (lds[0][threadIdx.x] + lds[1][threadIdx.x]) + (lds[2][threadIdx.x] + lds[3][threadIdx.x]);
+}
+
+// d_table[bucket][head]: a wave a (bucket, head)
+template <typename T>
+__global__ void __launch_bounds__(256) join_offsets_kernel(int heads, int offsets, int buckets, const int32_t* __restrict__ map,
+                                                           const double* __restrict__ d_offsets, void* __restrict__ d_table,
+                                                           int table_f32) {
+  const int bucket = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (bucket >= buckets) return;
+  for (int h = blockIdx.y; h < heads; h += gridDim.y) {
+    double t = 0;
+    for (int o = lane; o < offsets; o += 64)
+      if (map[o] == bucket) t += d_offsets[(int64_t)h * offsets + o];
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) t += __shfl_xor(t, m);
+    if (lane == 0) store_param<T>(d_table, table_f32, (int64_t)bucket * heads + h, (float)t);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+int count(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// codes that n neighbouring tokens span, less one, at most: a token a code, and gw - 1 more at the end of a row
+int span_of(int n, int gh, int gw) {
+  n = n < gh * gw ? n : gh * gw;
+  int crossings = count(n - 1, gw);
+  if (crossings > gh - 1) crossings = gh - 1;
+  return (n - 1) + crossings * (gw - 1);
+}
+
+struct Plan {
+  int waves, rows, tiles, splits, tiles_per_split, nq_pad, window, ring, ring_pitch, offsets, dp;
+  size_t part_o, part_ml, forward_total;
+  size_t delta, ring_rows, d_offsets, backward_total;
+};
+
+Plan plan(const PsRelativeAttentionDesc& d, bool training) {
+  Plan p = {};
+  const int nk = d.grid_h * d.grid_w, e = d.dtype == PS_DTYPE_F32 ? 4 : 2;
+  p.rows = e == 2 ? 64 : 32;
+  p.dp = d.dim <= 32 ? 32 : d.dim <= 64 ? 64 : 128;
+  p.offsets = (2 * d.grid_h - 1) * (2 * d.grid_w - 1);
+  p.nq_pad = count(d.queries, 64) * 64;
+  p.waves = d.queries <= 32 ? 1 : 4;
+  p.tiles = count(nk, p.rows);
+  const int64_t blocks = (int64_t)d.batch * d.heads * count(training ? p.nq_pad : d.queries, p.waves * 32);
+  // few blocks: split the keys, at least 4 tiles a split (a join reads and writes a row of o per split)
+  const int want = p.waves == 1 ? 1536 : 512;
+  p.splits = 1;
+  if (blocks < want / 2) {
+    int s = (int)(want / blocks);
+    if (s > p.tiles / 4) s = p.tiles / 4;
+    p.splits = s < 1 ? 1 : s;
+  }
+  p.tiles_per_split = count(p.tiles, p.splits);
+  p.splits = count(p.tiles, p.tiles_per_split);
+  const int cols = 128;      // at most
+  const int wide = span_of(cols, d.grid_h, d.grid_w) + span_of(p.rows, d.grid_h, d.grid_w) + 1;
+  p.window = count(wide, 64) * 64;
+  const int live = span_of(32, d.grid_h, d.grid_w) + span_of(p.rows, d.grid_h, d.grid_w) + 1;
+  p.ring = 64;
+  while (p.ring < live) p.ring *= 2;
+  p.ring_pitch = count((nk - 1) + (int64_t)(d.grid_h - 1) * (d.grid_w - 1) + span_of(32, d.grid_h, d.grid_w) + 1, 64) * 64;
+  const size_t rows = (size_t)d.batch * d.heads * d.queries;
+  size_t at = 0;
+  if (p.splits > 1) {
+    p.part_o = at; at += align256(sizeof(float) * p.splits * rows * d.dim);
+    p.part_ml = at; at += align256(sizeof(float) * p.splits * rows * 2);
+  }
+  p.forward_total = at + 256;
+  at = 0;
+  p.delta = at; at += align256(sizeof(float) * d.batch * d.heads * p.nq_pad);
+  p.ring_rows = at; at += align256(sizeof(float) * d.batch * d.heads * (p.nq_pad / 32) * p.ring_pitch);
+  p.d_offsets = at; at += align256(sizeof(double) * d.heads * p.offsets);
+  p.backward_total = at + 256;
+  return p;
+}
+
+Args args_of(const PsRelativeAttentionDesc& d, const Plan& p) {
+  Args a = {};
+  a.sq = {d.q_strides[0], d.q_strides[1], d.q_strides[2]};
+  a.sk = {d.k_strides[0], d.k_strides[1], d.k_strides[2]};
+  a.sv = {d.v_strides[0], d.v_strides[1], d.v_strides[2]};
+  a.sdo = {d.do_strides[0], d.do_strides[1], d.do_strides[2]};
+  a.mask_b = d.mask_stride;
+  a.batch = d.batch; a.heads = d.heads; a.nq = d.queries; a.nk = d.grid_h * d.grid_w; a.dim = d.dim;
+  a.gw = d.grid_w; a.origin = (d.grid_h - 1) * (2 * d.grid_w - 1) + d.grid_w - 1; a.offsets = p.offsets;
+  a.q_start = d.query_start; a.nq_pad = p.nq_pad; a.scale = d.scale * kLog2e; a.window = p.window;
+  a.ring = p.ring; a.ring_pitch = p.ring_pitch;
+  return a;
+}
+
+template <typename K>
+bool allow_lds(K kernel, size_t bytes) {
+  return bytes <= 64 * 1024 || hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                   hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == hipSuccess;
+}
+
+template <typename T, int DP, int WAVES>
+int run_forward(Args a, const Plan& p, hipStream_t st) {
+  a.col_tiles = count(a.stats ? a.nq_pad : a.nq, WAVES * 32);
+  a.splits = p.splits;
+  a.tiles_per_split = p.tiles_per_split;
+  const size_t lds = 2 * (size_t)Lds<T, DP, WAVES>::buffer(p.window);
+  auto kernel = attention_forward_kernel<T, DP, WAVES>;
+  if (!allow_lds(kernel, lds)) return PS_ERR_LAUNCH;
+  kernel<<<dim3((unsigned)(a.col_tiles * a.batch * a.heads), (unsigned)a.splits), WAVES * 64, lds, st>>>(a);
+  if (a.splits > 1) {
+    const int64_t items = (int64_t)a.batch * a.heads * a.nq_pad * (a.dim / 4);
+    join_splits_kernel<T><<<(unsigned)((items + 255) / 256), 256, 0, st>>>(a);
+  }
+  return PS_OK;
+}
+
+template <typename T, int DP>
+int run_backward(Args a, const Plan& p, bool table, hipStream_t st) {
+  constexpr int WAVES = 4;
+  const size_t lds = 2 * (size_t)Lds<T, DP, WAVES>::buffer(p.window);
+  const unsigned bh = (unsigned)(a.batch * a.heads);
+  a.col_tiles = count(a.nq_pad, WAVES * 32);
+  if (table) {
+    const size_t with = lds + (size_t)WAVES * p.ring * 4;
+    auto kernel = attention_dq_kernel<T, DP, WAVES, true>;
+    if (!allow_lds(kernel, with)) return PS_ERR_LAUNCH;
+    kernel<<<a.col_tiles * bh, WAVES * 64, with, st>>>(a);
+  } else {
+    auto kernel = attention_dq_kernel<T, DP, WAVES, false>;
+    if (!allow_lds(kernel, lds)) return PS_ERR_LAUNCH;
+    kernel<<<a.col_tiles * bh, WAVES * 64, lds, st>>>(a);
+  }
+  if (a.dk || a.dv) {
+    a.col_tiles = count(a.nk, WAVES * 32);
+    auto kernel = attention_dkv_kernel<T, DP, WAVES>;
+    if (!allow_lds(kernel, lds)) return PS_ERR_LAUNCH;
+    kernel<<<a.col_tiles * bh, WAVES * 64, lds, st>>>(a);
+  }
+  return PS_OK;
+}
+
+template <typename T>
+int forward_typed(const PsRelativeAttentionDesc& d, Args a, const Plan& p, const int32_t* map, const void* table,
+                  float* bias, hipStream_t st) {
+  spread_table_kernel<T><<<dim3((unsigned)count(p.offsets, 256), (unsigned)d.heads), 256, 0, st>>>(
+      d.heads, p.offsets, d.buckets, map, table, d.table_f32, bias);
+  if (p.waves == 1)
+    return p.dp == 32 ? run_forward<T, 32, 1>(a, p, st) : p.dp == 64 ? run_forward<T, 64, 1>(a, p, st)
+                                                                     : run_forward<T, 128, 1>(a, p, st);
+  return p.dp == 32 ? run_forward<T, 32, 4>(a, p, st) : p.dp == 64 ? run_forward<T, 64, 4>(a, p, st)
+                                                                   : run_forward<T, 128, 4>(a, p, st);
+}
+
+template <typename T>
+int backward_typed(const PsRelativeAttentionDesc& d, Args a, const Plan& p, const int32_t* map, void* d_table,
+                   double* d_offsets, hipStream_t st) {
+  const int rc = p.dp == 32 ? run_backward<T, 32>(a, p, d_table != nullptr, st)
+               : p.dp == 64 ? run_backward<T, 64>(a, p, d_table != nullptr, st)
+                            : run_backward<T, 128>(a, p, d_table != nullptr, st);
+  if (rc || !d_table) return rc;
+  join_rings_kernel<<<dim3((unsigned)count(p.offsets, 64), (unsigned)d.heads), 256, 0, st>>>(a, d_offsets);
+  join_offsets_kernel<T><<<dim3((unsigned)count(d.buckets, 4), (unsigned)d.heads), 256, 0, st>>>(
+      d.heads, p.offsets, d.buckets, map, d_offsets, d_table, d.table_f32);
+  return PS_OK;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int check(const PsRelativeAttentionDesc* d) {
+  if (!d || d->batch <= 0 || d->heads <= 0 || d->queries <= 0 || d->grid_h <= 0 || d->grid_w <= 0 || d->dim <= 0 ||
+      d->buckets <= 0 || d->query_start < 0)
+    return PS_ERR_BAD_ARG;
+  if (d->dtype < PS_DTYPE_F32 || d->dtype > PS_DTYPE_F16) return PS_ERR_UNSUPPORTED;
+  const int64_t nk = (int64_t)d->grid_h * d->grid_w;
+  if (nk > 1 << 20 || (d->grid_h > 1 && d->grid_w > 512) || d->dim > 128 || d->heads > 65535 ||
+      (int64_t)d->batch * d->heads > 1 << 24 || d->buckets > 1 << 24)
+    return PS_ERR_UNSUPPORTED;
+  if (d->query_start + (int64_t)d->queries > nk) return PS_ERR_BAD_ARG;
+  if ((int64_t)d->batch * d->heads * ((d->queries + 63) / 64 * 2) >= 1 << 30 ||
+      (int64_t)d->batch * d->heads * ((nk + 31) / 32) >= 1 << 30)
+    return PS_ERR_UNSUPPORTED;
+  const int chunk = d->dtype == PS_DTYPE_F32 ? 4 : 8;
+  if (d->dim % chunk) return PS_ERR_BAD_ARG;
+  return PS_OK;
+}
+// rows start on 16 bytes; 64 of them are within 32-bit offsets of each other
+int check_rows(const PsRelativeAttentionDesc& d, const void* p, const int64_t* strides) {
+  const int chunk = d.dtype == PS_DTYPE_F32 ? 4 : 8;
+  if (!p || !aligned16(p)) return PS_ERR_BAD_ARG;
+  for (int i = 0; i < 3; ++i)
+    if (strides[i] % chunk || strides[i] < 0) return PS_ERR_BAD_ARG;
+  return strides[2] < (int64_t)1 << 24 ? PS_OK : PS_ERR_UNSUPPORTED;
+}
+
+}  // namespace
+}  // namespace ps
+
+using namespace ps;
+
+extern "C" {
+
+size_t ps_relative_attention_workspace_bytes(const PsRelativeAttentionDesc* d, int32_t backward) {
+  if (check(d)) return 0;
+  if (backward) return plan(*d, true).backward_total;
+  const size_t a = plan(*d, false).forward_total, b = plan(*d, true).forward_total;
+  return a > b ? a : b;
+}
+
+int ps_relative_attention_forward(const PsRelativeAttentionDesc* d, const void* q, const void* k, const void* v,
+                                  const uint8_t* key_mask, const int32_t* bucket_map, const void* table, void* out,
+                                  float* out_f32, float* stats, float* bias, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+  if (int rc = check(d)) return rc;
+  if (int rc = check_rows(*d, q, d->q_strides)) return rc;
+  if (int rc = check_rows(*d, k, d->k_strides)) return rc;
+  if (int rc = check_rows(*d, v, d->v_strides)) return rc;
+  if (!bucket_map || !table || !out || !aligned16(out) || !bias || !workspace || !aligned16(workspace) ||
+      (out_f32 && !aligned16(out_f32)))
+    return PS_ERR_BAD_ARG;
+  if (workspace_bytes < ps_relative_attention_workspace_bytes(d, 0)) return PS_ERR_WORKSPACE;
+  const Plan p = plan(*d, stats != nullptr);
+  Args a = args_of(*d, p);
+  a.q = q; a.k = k; a.v = v; a.mask = key_mask; a.bias = bias;
+  a.out = out; a.o32 = out_f32; a.stats = stats;
+  a.part_o = (float*)((char*)workspace + p.part_o);
+  a.part_ml = (float*)((char*)workspace + p.part_ml);
+  hipStream_t st = (hipStream_t)stream;
+  int rc;
+  switch (d->dtype) {
+    case PS_DTYPE_F32: rc = forward_typed<float>(*d, a, p, bucket_map, table, bias, st); break;
+    case PS_DTYPE_BF16: rc = forward_typed<bf16>(*d, a, p, bucket_map, table, bias, st); break;
+    default: rc = forward_typed<f16>(*d, a, p, bucket_map, table, bias, st); break;
+  }
+  return rc ? rc : hipGetLastError() == hipSuccess ? PS_OK : PS_ERR_LAUNCH;
+}
+
+int ps_relative_attention_backward(const PsRelativeAttentionDesc* d, const void* q, const void* k, const void* v,
+                                   const uint8_t* key_mask, const int32_t* bucket_map, const float* bias,
+                                   const float* out_f32, const float* stats, const void* d_out, void* dq, void* dk, void* dv,
+                                   void* d_table, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check(d)) return rc;
+  if (int rc = check_rows(*d, q, d->q_strides)) return rc;
+  if (int rc = check_rows(*d, k, d->k_strides)) return rc;
+  if (int rc = check_rows(*d, v, d->v_strides)) return rc;
+  if (int rc = check_rows(*d, d_out, d->do_strides)) return rc;
+  if (!bucket_map || !bias || !out_f32 || !stats || !workspace || !aligned16(workspace)) return PS_ERR_BAD_ARG;
+  if (!aligned16(dq) || !aligned16(dk) || !aligned16(dv)) return PS_ERR_BAD_ARG;
+  if (workspace_bytes < ps_relative_attention_workspace_bytes(d, 1)) return PS_ERR_WORKSPACE;
+  const Plan p = plan(*d, true);
+  Args a = args_of(*d, p);
+  char* ws = (char*)workspace;
+  a.q = q; a.k = k; a.v = v; a.mask = key_mask; a.bias = bias; a.dout = d_out;
+  a.o_kept = out_f32; a.stats = const_cast<float*>(stats); a.delta = (float*)(ws + p.delta);
+  a.ring_rows = (float*)(ws + p.ring_rows);
+  a.dq = dq; a.dk = dk; a.dv = dv;
+  double* d_offsets = (double*)(ws + p.d_offsets);
+  hipStream_t st = (hipStream_t)stream;
+  int rc;
+  switch (d->dtype) {
+    case PS_DTYPE_F32: rc = backward_typed<float>(*d, a, p, bucket_map, d_table, d_offsets, st); break;
+    case PS_DTYPE_BF16: rc = backward_typed<bf16>(*d, a, p, bucket_map, d_table, d_offsets, st); break;
+    default: rc = backward_typed<f16>(*d, a, p, bucket_map, d_table, d_offsets, st); break;
+  }
+  return rc ? rc : hipGetLastError() == hipSuccess ? PS_OK : PS_ERR_LAUNCH;
+}
+
+}  // extern "C"

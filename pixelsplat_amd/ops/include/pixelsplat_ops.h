@@ -70,6 +70,37 @@ int ps_gated_linear_backward(const PsGatedLinearDesc* desc, const void* x, const
                              void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, void* workspace,
                              size_t workspace_bytes, void* stream);
 
+/* Attention over a grid of grid_h x grid_w tokens (numbered by rows) with a learned relative position bias:
+ *   s = scale q.k + table[bucket_map[key row - query row + grid_h - 1][key column - query column + grid_w - 1]][head]
+ *   out = softmax(s over the keys whose key_mask is not 0) v; a row without keys is zero.
+ * The queries are the tokens query_start .. query_start + queries - 1, the keys and values all tokens.  q, k, v, d_out
+ * are read at strides (batch, head, token; elements, unit stride within a row of dim); their rows start on 16 bytes
+ * and hold whole 16-byte chunks.  out, dq [batch][queries][heads][dim] and dk, dv [batch][keys][heads][dim] are
+ * contiguous.  key_mask [batch][keys] bytes or NULL: the rows of k and v of masked keys are not read.  bucket_map
+ * [2 grid_h - 1][2 grid_w - 1]; an entry outside 0 .. buckets - 1 is an offset without bias.  table [buckets][heads] in
+ * the tensors' type, or fp32 when table_f32.
+ * For the backward the forward leaves bias [heads][offsets] fp32 (always written), stats [2][batch][heads][queries
+ * rounded up to 64] fp32 and out_f32 (the unrounded out; fp32 tensors hand `out` itself to the backward and NULL to the
+ * forward); stats and out_f32 are NULL where no backward follows.  Backward: each output may be NULL.
+ * dim <= 128, keys <= 2^20, grid_w <= 512 unless grid_h is 1, token strides < 2^24 (else PS_ERR_UNSUPPORTED). */
+typedef struct PsRelativeAttentionDesc {
+  int32_t batch, heads, queries, query_start, grid_h, grid_w, dim;
+  int32_t dtype, buckets, table_f32;
+  float scale;
+  int32_t reserved; /* 0 */
+  int64_t q_strides[3], k_strides[3], v_strides[3], do_strides[3];
+  int64_t mask_stride; /* of a batch element */
+} PsRelativeAttentionDesc;
+size_t ps_relative_attention_workspace_bytes(const PsRelativeAttentionDesc* desc, int32_t backward);
+int ps_relative_attention_forward(const PsRelativeAttentionDesc* desc, const void* q, const void* k, const void* v,
+                                  const uint8_t* key_mask, const int32_t* bucket_map, const void* table, void* out,
+                                  float* out_f32, float* stats, float* bias, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+int ps_relative_attention_backward(const PsRelativeAttentionDesc* desc, const void* q, const void* k, const void* v,
+                                   const uint8_t* key_mask, const int32_t* bucket_map, const float* bias,
+                                   const float* out_f32, const float* stats, const void* d_out, void* dq, void* dk, void* dv,
+                                   void* d_table, void* workspace, size_t workspace_bytes, void* stream);
+
 /* "pixelsplat_ops gfx950 | <file>:<hash> ...", as ps_build_info of pixelsplat_hip.h. */
 const char* ps_ops_build_info(void);
 

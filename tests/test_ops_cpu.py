@@ -146,3 +146,103 @@ def test_gated_linear_c_abi_refusals(lib):
         assert forward(bad) == status and backward(bad) == status, field
         assert lib.ps_gated_linear_backward_workspace_bytes(C.byref(bad)) == 0
     assert backward(_lib.PsGatedLinearDesc(**{**good, "dh_row_stride": 4})) == -1
+
+
+def _attention_args(**changes):
+    fake = lambda *s, dtype=torch.float32: _FakeGpu(torch.zeros(s, dtype=dtype))  # noqa: E731
+    a = dict(q=fake(2, 3, 6, 8), k=fake(2, 3, 6, 8), v=fake(2, 3, 6, 8), table=fake(5, 3),
+             buckets=fake(3, 5, dtype=torch.int32))
+    return {**a, **{n: fake(*c) if isinstance(c, tuple) else c for n, c in changes.items()}}
+
+
+@pytest.mark.parametrize("changes,match", [
+    (dict(k=(2, 3, 7, 8)), "q .batch"), (dict(q=(2, 3, 6)), "q .batch"), (dict(q=(2, 4, 6, 8)), "q .batch"),
+    (dict(q=(2, 3, 6, 16)), "q .batch"), (dict(k=(2, 3, 7, 8), v=(2, 3, 7, 8)), "7 keys on a grid of 2 x 3"),
+    (dict(q=(2, 3, 7, 8)), "queries 0 .. 6 of 6"), (dict(query_start=1), "queries 1 .. 6"), (dict(query_start=-1), "queries -1"),
+    (dict(table=(5, 2)), "table is"), (dict(table=(0, 3)), "table is"), (dict(table=(3,)), "table is"),
+    (dict(buckets=(3, 5)), "int32"), (dict(key_mask=(2, 6)), "bool")])
+def test_relative_attention_refusals(lib, changes, match):
+    from pixelsplat_amd.ops import relative_attention
+    with pytest.raises(ValueError, match=match):
+        relative_attention(**_attention_args(**changes))
+
+
+def test_relative_attention_more_refusals(lib):
+    from pixelsplat_amd.ops import RelativePositionBias, relative_attention, relative_buckets
+    fake = lambda *s, dtype=torch.float32: _FakeGpu(torch.zeros(s, dtype=dtype))  # noqa: E731
+    with pytest.raises(ValueError, match="buckets is"):
+        relative_attention(**_attention_args(buckets=fake(4, 5, dtype=torch.int32)))
+    with pytest.raises(ValueError, match="k and v are"):
+        relative_attention(**_attention_args(v=fake(2, 3, 6, 8, dtype=torch.bfloat16)))
+    with pytest.raises(ValueError, match="dim 136"):
+        relative_attention(**_attention_args(q=(2, 3, 6, 136), k=(2, 3, 6, 136), v=(2, 3, 6, 136)))
+    wide = dict(q=fake(1, 1, 1, 1), k=fake(1, 1, 1026, 1), v=fake(1, 1, 1026, 1), table=fake(5, 1),
+                buckets=fake(3, 1025, dtype=torch.int32))
+    with pytest.raises(ValueError, match="512 columns"):
+        relative_attention(**wide)
+    with pytest.raises(RuntimeError, match="table is on"):
+        relative_attention(**_attention_args(table=torch.zeros(5, 3)))
+    x = torch.zeros(1, 1, 1, 8)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        relative_attention(x, x, x, torch.zeros(1, 1), torch.zeros(1, 1, dtype=torch.int32))
+    for bad in (0, 6, -4):
+        with pytest.raises(ValueError, match="multiple of 4"):
+            RelativePositionBias(2, bad)
+    with pytest.raises(ValueError, match="max_distance"):
+        relative_buckets((4, 4), 32, 8)
+    with pytest.raises(ValueError, match="at least one row"):
+        relative_buckets((0, 4))
+
+
+def test_relative_buckets():
+    from pixelsplat_amd.ops import RelativePositionBias, relative_bucket_count, relative_buckets
+    b = relative_buckets((1, 300), 32, 128)[0]
+    at = lambda d: int(b[d + 299])  # noqa: E731
+    assert [at(-d) for d in range(8)] == list(range(8)) and [at(d) for d in range(1, 8)] == list(range(17, 24))
+    assert at(-8) == 8 and at(-15) == 9 and at(-16) == 10 and at(-299) == at(-128) == 15 and at(128) == at(299) == 31
+    # far distances 8 16^(j / 8): 8, 11.3, 16, 22.6, 32, 45.3, 64, 90.5
+    assert [at(-d) for d in (11, 12, 22, 23, 31, 32, 45, 46, 63, 64, 90, 91)] == [8, 9, 10, 11, 11, 12, 12, 13, 13, 14, 14, 15]
+    two = relative_buckets((3, 4), 8)
+    assert two.shape == (5, 7) and two.dtype == torch.int32
+    assert int(two[2, 3]) == 0 and int(two[2, 4]) == 5 and int(two[3, 3]) == 40 and int(two[0, 0]) == 2 * 8 + 2
+    assert int(two.max()) < relative_bucket_count((3, 4), 8) == 64
+    assert relative_bucket_count((1, 9)) == relative_bucket_count((9, 1)) == 32 and relative_bucket_count((1, 1)) == 1
+    net = RelativePositionBias(2, 8)
+    assert torch.equal(net.buckets((3, 4), "cpu"), two) and net.buckets((3, 4), "cpu") is net.buckets((3, 4), "cpu")
+    assert torch.equal(net.buckets((1, 9), "cpu"), relative_buckets((1, 9), 8)) and list(net.state_dict()) == ["table"]
+
+
+def test_relative_attention_c_abi_refusals(lib):
+    from pixelsplat_amd.ops import _lib
+    three = C.c_int64 * 3
+    s = three(96, 8, 24)
+    good = dict(batch=2, heads=1, queries=6, query_start=0, grid_h=2, grid_w=3, dim=8, dtype=1, buckets=5, table_f32=0,
+                scale=0.3, reserved=0, q_strides=s, k_strides=s, v_strides=s, do_strides=s, mask_stride=6)
+    p = 4096          # an address that is never followed
+    ok = _lib.PsRelativeAttentionDesc(**good)
+    assert lib.ps_relative_attention_workspace_bytes(C.byref(ok), 0) > 0
+    assert lib.ps_relative_attention_workspace_bytes(C.byref(ok), 1) > 0
+
+    def forward(d, q=p, table=p, out=p, bias=p, ws=p, n=1 << 40):
+        return lib.ps_relative_attention_forward(C.byref(d) if d else None, q, p, p, None, p, table, out, None, None, bias,
+                                                 ws, n, None)
+
+    def backward(d, stats=p, do=p, dq=p, ws=p, n=1 << 40):
+        return lib.ps_relative_attention_backward(C.byref(d) if d else None, p, p, p, None, p, p, p, stats, do, dq, None,
+                                                  None, None, ws, n, None)
+
+    assert forward(None) == backward(None) == -1
+    assert forward(ok, q=None) == forward(ok, q=p + 2) == forward(ok, table=None) == forward(ok, out=p + 8) == -1
+    assert forward(ok, bias=None) == forward(ok, ws=None) == backward(ok, stats=None) == backward(ok, do=p + 2) == -1
+    assert backward(ok, dq=p + 4) == backward(ok, ws=p + 4) == -1
+    assert forward(ok, n=10) == backward(ok, n=10) == -2
+    for field, value, status in [("batch", 0, -1), ("heads", -1, -1), ("queries", 0, -1), ("queries", 7, -1),
+                                 ("query_start", 1, -1), ("query_start", -1, -1), ("grid_h", 0, -1), ("dim", 12, -1),
+                                 ("dim", 136, -4), ("dtype", 3, -4), ("buckets", 0, -1), ("grid_w", 1024, -4),
+                                 ("grid_h", 1 << 20, -4)]:
+        bad = _lib.PsRelativeAttentionDesc(**{**good, field: value})
+        assert forward(bad) == status and backward(bad) == status, field
+        assert lib.ps_relative_attention_workspace_bytes(C.byref(bad), 1) == 0
+    for strides, status in [(three(96, 8, 20), -1), (three(-96, 8, 24), -1), (three(96, 8, 1 << 24), -4)]:
+        assert forward(_lib.PsRelativeAttentionDesc(**{**good, "k_strides": strides})) == status
+        assert backward(_lib.PsRelativeAttentionDesc(**{**good, "do_strides": strides})) == status
