@@ -1,22 +1,18 @@
-"""ctypes binding of libpixelsplat_ops.so (the C ABI of pixelsplat_ops.h) and what its operators share: the checks of
-their arguments, the launch on a tensor's own device and the status codes.  No fallback: a missing library raises."""
+"""libpixelsplat_ops.so (the C ABI of pixelsplat_ops.h, through ctypes) and _binding.so (the same operators as torch
+functions: what the package calls).  No fallback: a missing library raises."""
 from __future__ import annotations
 
 import ctypes as C
 import os
 
-import torch
-from torch import Tensor
+import torch  # noqa: F401  (its HIP runtime has to be in the process before the library is)
 
 from .._lib import HipExtensionMissing
 
 LIB_PATH = os.environ.get("PIXELSPLAT_OPS_LIB") or os.path.join(
     os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "libpixelsplat_ops.so")
 
-DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "sigmoid": 4}
-STATUS = {-1: "bad argument (null or misaligned pointer, inconsistent descriptor)", -2: "workspace too small",
-          -3: "HIP launch failed", -4: "unsupported configuration"}
 
 
 class PsGroupNormDesc(C.Structure):
@@ -53,6 +49,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_binding = None
 
 
 def load():
@@ -63,7 +60,7 @@ def load():
     if not os.path.exists(LIB_PATH):
         raise HipExtensionMissing(f"{LIB_PATH} not found: build it with `python -m pixelsplat_amd.ops.build` "
                                   "(hipcc --offload-arch=gfx950). There is no non-HIP fallback for these operators.")
-    lib = C.CDLL(LIB_PATH)          # torch is imported above: both resolve to the HIP runtime it ships
+    lib = C.CDLL(LIB_PATH)
     for name, (result, arguments) in SIGNATURES.items():
         if not hasattr(lib, name):
             raise HipExtensionMissing(f"{LIB_PATH} does not export {name}")
@@ -73,35 +70,21 @@ def load():
     return lib
 
 
-def call(name: str, device: torch.device, *args) -> None:
-    """lib.name(*args, stream) on `device` and its current stream; tensors become pointers, a status becomes an error."""
-    fn = getattr(_lib or load(), name)
-    args = [a.data_ptr() if isinstance(a, Tensor) else a for a in args]
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
-    if rc:
-        raise RuntimeError(f"{name} failed: {STATUS.get(rc, 'unknown status')} (PsStatus {rc})")
+def binding():
+    """The operators as torch functions (_binding.so, csrc/binding.cpp): cached, and as loud when it is missing."""
+    global _binding
+    if _binding is None:
+        load()
+        try:
+            from . import _binding as module
+        except ImportError as e:
+            raise HipExtensionMissing(f"pixelsplat_amd/ops/_binding.so is missing or does not load ({e}): build it with "
+                                      "`python -m pixelsplat_amd.ops.build`. There is no fallback.") from e
+        _binding = module
+    return _binding
 
 
-def check_tensors(op: str, first: Tensor, **others: Tensor | None) -> None:
-    """`first` is a GPU tensor of a supported type; every other tensor is on its device."""
-    if first.dtype not in DTYPES:
-        raise TypeError(f"{op}: fp32, bf16 or fp16 tensors, got {first.dtype}")
-    if not first.is_cuda:
-        raise RuntimeError(f"{op} needs GPU tensors (no CPU fallback)")
-    for name, t in others.items():
-        if t is not None and t.device != first.device:
-            raise RuntimeError(f"{op}: {name} is on {t.device}, the input on {first.device}")
-
-
-def activation_code(op: str, name: str, allowed=tuple(ACTIVATIONS)) -> int:
-    if name not in allowed:
-        raise ValueError(f"{op}: activation {name!r} is none of {', '.join(allowed)}")
+def activation_code(op: str, name: str) -> int:
+    if name not in ACTIVATIONS:
+        raise ValueError(f"{op}: activation {name!r} is none of {', '.join(ACTIVATIONS)}")
     return ACTIVATIONS[name]
-
-
-def wants_grad(*tensors: Tensor | None) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)

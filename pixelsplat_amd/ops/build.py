@@ -1,4 +1,5 @@
-"""Builds libpixelsplat_ops.so in-tree with hipcc for gfx950 (cross-compiles without a GPU).
+"""Builds libpixelsplat_ops.so in-tree with hipcc for gfx950 (cross-compiles without a GPU), and _binding.so, the
+operators as torch functions over it, with the host's compiler.
 
     python -m pixelsplat_amd.ops.build [--force] [--verbose]
 
@@ -11,6 +12,7 @@ import hashlib
 import os
 import subprocess
 import sys
+import sysconfig
 
 from ..build import _hipcc
 
@@ -18,6 +20,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PACKAGE = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(PACKAGE, "libpixelsplat_ops.so")
+BINDING = os.path.join(HERE, "_binding.so")
 HEADERS = [os.path.join(HERE, "include", "pixelsplat_ops.h"),
            os.path.join(os.path.dirname(PACKAGE), "include", "pixelsplat_hip.h")]
 INFO_UNIT = "ops_info.hip"      # carries every unit's hash (ps_ops_build_info)
@@ -80,7 +83,36 @@ def build(force: bool = False, verbose: bool = False) -> str:
         raise RuntimeError("\n".join(failed))
     if procs or not os.path.exists(LIB):
         subprocess.check_call([_hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-o", LIB])
+    build_binding(force, verbose)
     return LIB
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> str:
+    import torch
+    from torch.utils import cpp_extension
+
+    src = os.path.join(CSRC, "binding.cpp")
+    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__"]
+    stamp = hashlib.sha256(" ".join([*flags, torch.__version__, sys.version]).encode())
+    for path in [src, *HEADERS]:
+        stamp.update(open(path, "rb").read())
+    mark = os.path.join(CSRC, "binding.o.tmp")
+    if not force and os.path.exists(BINDING) and os.path.exists(mark) and open(mark).read() == stamp.hexdigest():
+        return BINDING
+    cmd = ["g++", *flags, src, "-o", BINDING]
+    cmd += [x for h in HEADERS for x in ("-I", os.path.dirname(h))]
+    cmd += [x for d in [*cpp_extension.include_paths(), "/opt/rocm/include", sysconfig.get_paths()["include"]]
+            for x in ("-isystem", d)]
+    cmd += [x for d in cpp_extension.library_paths() for x in ("-L", d)] + ["-L", PACKAGE]
+    cmd += ["-lpixelsplat_ops", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-ltorch_python", "-Wl,-rpath,$ORIGIN/.."]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on binding.cpp:\n{r.stdout}")
+    with open(mark, "w") as f:
+        f.write(stamp.hexdigest())
+    return BINDING
 
 
 if __name__ == "__main__":
