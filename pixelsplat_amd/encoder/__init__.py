@@ -9,4 +9,5 @@ from .epipolar_sampler import EpipolarSampler, EpipolarSampling  # noqa: F401
 from .epipolar_transformer import (EpipolarTransformer, EpipolarTransformerCfg,  # noqa: F401
                                    ImageSelfAttentionCfg)
 from .gaussian_adapter import GaussianAdapter, GaussianAdapterCfg, Gaussians  # noqa: F401
-from .transformer import Attention, FeedForward, PreNorm, Transformer  # noqa: F401
+from .transformer import (Attention, FeedForward, GatedFeedForward, PreNorm,  # noqa: F401
+                          Transformer)

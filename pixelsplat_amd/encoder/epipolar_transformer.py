@@ -21,8 +21,9 @@ from torch import Tensor, nn
 
 from ..epipolar import (FeatureGradBatch, fold_attention_weights, fused_cross_attention,
                         gather_features, layer_norm, layer_norm_fork)
+from ..ops import GroupNormAct
 from .epipolar_sampler import EpipolarSampler, EpipolarSampling
-from .transformer import Transformer
+from .transformer import FeedForward, GatedFeedForward, Transformer
 
 
 @dataclass
@@ -34,6 +35,11 @@ class ImageSelfAttentionCfg:
     d_token: int
     d_dot: int
     d_mlp: int
+    # beyond the reference (0 / False: its modules exactly): buckets an axis of a learned relative position bias on the
+    # patch grid, a gated projection in the feed-forward, groups of a group norm before the patches' activation
+    relative_buckets: int = 0
+    gated_mlp: bool = False
+    norm_groups: int = 0
 
 
 @dataclass
@@ -46,6 +52,7 @@ class EpipolarTransformerCfg:
     d_dot: int
     d_mlp: int
     downscale: int
+    refinement_groups: int = 0   # beyond the reference: a group norm before the refinement's activation
 
 
 class PositionalEncoding(nn.Module):
@@ -71,12 +78,18 @@ class PositionalEncoding(nn.Module):
 class ImageSelfAttention(nn.Module):
     def __init__(self, cfg: ImageSelfAttentionCfg, d_in: int, d_out: int):
         super().__init__()
+        # the reference's own configuration objects do not have these
+        relative_buckets, norm_groups = getattr(cfg, "relative_buckets", 0), getattr(cfg, "norm_groups", 0)
+        gated_mlp = getattr(cfg, "gated_mlp", False)
         self.positional_encoding = nn.Sequential(
             (pe := PositionalEncoding(cfg.num_octaves)), nn.Linear(pe.d_out(2), cfg.d_token))
         self.patch_embedder = nn.Sequential(
-            nn.Conv2d(d_in, cfg.d_token, cfg.patch_size, cfg.patch_size), nn.ReLU())
+            nn.Conv2d(d_in, cfg.d_token, cfg.patch_size, cfg.patch_size),
+            GroupNormAct(norm_groups, cfg.d_token, activation="relu") if norm_groups else nn.ReLU())
+        self.relative = relative_buckets > 0
         self.transformer = Transformer(cfg.d_token, cfg.num_layers, cfg.num_heads, cfg.d_dot,
-                                       cfg.d_mlp)
+                                       cfg.d_mlp, relative_buckets=relative_buckets,
+                                       feed_forward_layer=GatedFeedForward if gated_mlp else FeedForward)
         self.resampler = nn.ConvTranspose2d(cfg.d_token, d_out, cfg.patch_size, cfg.patch_size)
 
     def forward(self, image: Tensor) -> Tensor:
@@ -87,7 +100,7 @@ class ImageSelfAttention(nn.Module):
         xy = torch.stack(((xs + 0.5) / nw, (ys + 0.5) / nh), -1).float()
         tokens = tokens + self.positional_encoding(xy).permute(2, 0, 1)
         b, c = tokens.shape[:2]
-        tokens = self.transformer(tokens.flatten(2).transpose(1, 2))
+        tokens = self.transformer(tokens.flatten(2).transpose(1, 2), grid=(nh, nw) if self.relative else None)
         tokens = tokens.transpose(1, 2).reshape(b, c, nh, nw)
         return self.resampler(tokens)
 
@@ -138,8 +151,11 @@ class EpipolarTransformer(nn.Module):
         if cfg.downscale:
             self.downscaler = nn.Conv2d(d_in, d_in, cfg.downscale, cfg.downscale)
             self.upscaler = nn.ConvTranspose2d(d_in, d_in, cfg.downscale, cfg.downscale)
+            groups = getattr(cfg, "refinement_groups", 0)
             self.upscale_refinement = nn.Sequential(
-                nn.Conv2d(d_in, d_in * 2, 7, 1, 3), nn.GELU(), nn.Conv2d(d_in * 2, d_in, 7, 1, 3))
+                nn.Conv2d(d_in, d_in * 2, 7, 1, 3),
+                GroupNormAct(groups, d_in * 2, activation="gelu") if groups else nn.GELU(),
+                nn.Conv2d(d_in * 2, d_in, 7, 1, 3))
         if num_context_views > 2:
             self.view_embeddings = nn.Embedding(num_context_views, d_in)
 

@@ -1,13 +1,17 @@
 """Attention / PreNorm / FeedForward / Transformer with the reference's parameter names and
-call conventions (/root/reference/src/model/transformer/{attention,pre_norm,feed_forward,
-transformer}.py, vendored there from stelzner/srt).  Plain PyTorch: the dense projections are
-library GEMMs; the epipolar cross-attention is routed to the fused HIP kernel by
-EpipolarTransformer, everything else (self-attention over 256 tokens / image) is out of the
-hot path."""
+call conventions (src/model/transformer/{attention,pre_norm,feed_forward,transformer}.py,
+vendored there from stelzner/srt).  Plain PyTorch: the dense projections are library GEMMs; the
+epipolar cross-attention is routed to the fused HIP kernel by EpipolarTransformer.
+
+Beyond the reference, off by default: `relative_buckets` gives self-attention over a token grid a
+learned relative position bias (ops.relative_attention), and GatedFeedForward is a feed-forward
+layer with a gated projection (ops.gated_linear)."""
 from __future__ import annotations
 
 import torch
 from torch import nn
+
+from ..ops import RelativePositionBias, gated_linear
 
 
 class FeedForward(nn.Module):
@@ -18,6 +22,23 @@ class FeedForward(nn.Module):
 
     def forward(self, x):
         return self.net(x)
+
+
+class GatedFeedForward(nn.Module):
+    """FeedForward with a gated projection: down(act(x w_gate^T + b_gate) * (x w_up^T + b_up)), the
+    bracket one kernel (ops.gated_linear: no projection reaches memory in 16-bit types)."""
+
+    def __init__(self, dim, hidden_dim, dropout=0.0, activation="silu", bias=True):
+        super().__init__()
+        self.activation = activation
+        self.gate = nn.Linear(dim, hidden_dim, bias=bias)
+        self.up = nn.Linear(dim, hidden_dim, bias=bias)
+        self.down = nn.Linear(hidden_dim, dim, bias=bias)
+        self.dropout = nn.Dropout(dropout)
+
+    def forward(self, x):
+        h = gated_linear(x, self.gate.weight, self.up.weight, self.gate.bias, self.up.bias, self.activation)
+        return self.dropout(self.down(self.dropout(h)))
 
 
 class PreNorm(nn.Module):
@@ -31,7 +52,12 @@ class PreNorm(nn.Module):
 
 
 class Attention(nn.Module):
-    def __init__(self, dim, heads=8, dim_head=64, dropout=0.0, selfatt=True, kv_dim=None):
+    """relative_buckets > 0 (self-attention only): a learned bias on the tokens' offsets on a grid,
+    relative_buckets logarithmic buckets an axis.  forward then takes the grid (rows, columns) of the
+    tokens, and a key mask [batch, tokens] for padded batches."""
+
+    def __init__(self, dim, heads=8, dim_head=64, dropout=0.0, selfatt=True, kv_dim=None,
+                 relative_buckets=0):
         super().__init__()
         inner_dim = dim_head * heads
         project_out = not (heads == 1 and dim_head == dim)
@@ -43,10 +69,15 @@ class Attention(nn.Module):
         else:
             self.to_q = nn.Linear(dim, inner_dim, bias=False)
             self.to_kv = nn.Linear(kv_dim, inner_dim * 2, bias=False)
+        if relative_buckets and not selfatt:
+            raise ValueError("a relative position bias needs self-attention: keys on the queries' grid")
+        self.relative_bias = RelativePositionBias(heads, relative_buckets) if relative_buckets else None
         self.to_out = (nn.Sequential(nn.Linear(inner_dim, dim), nn.Dropout(dropout))
                        if project_out else nn.Identity())
 
-    def forward(self, x, z=None):
+    def forward(self, x, z=None, grid=None, key_mask=None):
+        if (grid is None) != (self.relative_bias is None) or (key_mask is not None and grid is None):
+            raise ValueError("a grid (and with it a key mask) goes with relative_buckets, and only with it")
         if z is None:
             q, k, v = self.to_qkv(x).chunk(3, dim=-1)
         else:
@@ -54,25 +85,37 @@ class Attention(nn.Module):
             k, v = self.to_kv(z).chunk(2, dim=-1)
         split = lambda t: t.reshape(t.shape[0], t.shape[1], self.heads, -1).transpose(1, 2)
         q, k, v = split(q), split(k), split(v)
-        attn = self.attend(torch.matmul(q, k.transpose(-1, -2)) * self.scale)
-        out = torch.matmul(attn, v).transpose(1, 2)
+        if self.relative_bias is not None and len(self.attend._forward_hooks) == 0:
+            out = self.relative_bias(q, k, v, grid, key_mask, self.scale).transpose(1, 2)
+        else:   # a hook on `attend` sees the attention weights
+            logits = torch.matmul(q, k.transpose(-1, -2)) * self.scale
+            if grid is not None:
+                logits = logits + self.relative_bias.matrix(grid).to(logits.dtype)
+            if key_mask is not None:
+                logits = logits.masked_fill(~key_mask[:, None, None], float("-inf"))
+            attn = self.attend(logits)
+            if key_mask is not None:      # rows without keys
+                attn = torch.where(key_mask.any(1)[:, None, None, None], attn, torch.zeros_like(attn))
+                v = torch.where(key_mask[:, None, :, None], v, torch.zeros_like(v))
+            out = torch.matmul(attn, v).transpose(1, 2)
         return self.to_out(out.reshape(out.shape[0], out.shape[1], -1))
 
 
 class Transformer(nn.Module):
     def __init__(self, dim, depth, heads, dim_head, mlp_dim, dropout=0.0, selfatt=True,
-                 kv_dim=None, feed_forward_layer=FeedForward):
+                 kv_dim=None, feed_forward_layer=FeedForward, relative_buckets=0):
         super().__init__()
         self.layers = nn.ModuleList([])
         for _ in range(depth):
             self.layers.append(nn.ModuleList([
                 PreNorm(dim, Attention(dim, heads=heads, dim_head=dim_head, dropout=dropout,
-                                       selfatt=selfatt, kv_dim=kv_dim)),
+                                       selfatt=selfatt, kv_dim=kv_dim,
+                                       relative_buckets=relative_buckets)),
                 PreNorm(dim, feed_forward_layer(dim, mlp_dim, dropout=dropout)),
             ]))
 
-    def forward(self, x, z=None, **kwargs):
+    def forward(self, x, z=None, grid=None, key_mask=None, **kwargs):
         for attn, ff in self.layers:
-            x = attn(x, z=z) + x
+            x = attn(x, z=z, grid=grid, key_mask=key_mask) + x
             x = ff(x, **kwargs) + x
         return x

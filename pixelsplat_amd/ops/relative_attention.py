@@ -83,6 +83,13 @@ class RelativePositionBias(nn.Module):
             self._maps[key] = (rows[:, None] * self.buckets_per_axis + cols[None]).int().to(device)
         return self._maps[key]
 
+    def matrix(self, grid: tuple[int, int]) -> Tensor:
+        """[heads, tokens, tokens]: the bias written out, for what has to see the attention weights."""
+        gh, gw = _grid(grid)
+        at = torch.arange(gh * gw, device=self.table.device)
+        rows, cols = (at // gw)[None] - (at // gw)[:, None], (at % gw)[None] - (at % gw)[:, None]
+        return self.table[self.buckets(grid, self.table.device).long()[rows + gh - 1, cols + gw - 1]].permute(2, 0, 1)
+
     def forward(self, q: Tensor, k: Tensor, v: Tensor, grid: tuple[int, int], key_mask: Optional[Tensor] = None,
                 scale: Optional[float] = None, query_start: int = 0) -> Tensor:
         return relative_attention(q, k, v, self.table, self.buckets(grid, q.device), key_mask, scale, query_start)

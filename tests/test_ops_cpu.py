@@ -239,3 +239,29 @@ def test_relative_attention_c_abi_refusals(lib):
     for strides, status in [(three(96, 8, 20), -1), (three(-96, 8, 24), -1), (three(96, 8, 1 << 24), -4)]:
         assert forward(_lib.PsRelativeAttentionDesc(**{**good, "k_strides": strides})) == status
         assert backward(_lib.PsRelativeAttentionDesc(**{**good, "do_strides": strides})) == status
+
+
+def test_encoder_modules_take_the_operators_when_asked(lib):
+    """The options' modules and parameters; configuration objects without them (the reference's own) give the reference's."""
+    from types import SimpleNamespace
+
+    from pixelsplat_amd.encoder import (Attention, EpipolarTransformer, EpipolarTransformerCfg, FeedForward,
+                                        GatedFeedForward, ImageSelfAttentionCfg)
+    sa = dict(patch_size=2, num_octaves=4, num_layers=1, num_heads=2, d_token=16, d_dot=8, d_mlp=32)
+    et = dict(num_octaves=10, num_layers=1, num_heads=2, num_samples=4, d_dot=8, d_mlp=32, downscale=2)
+    plain = EpipolarTransformer(EpipolarTransformerCfg(self_attention=ImageSelfAttentionCfg(**sa), **et), 16, 2)
+    bare = EpipolarTransformer(SimpleNamespace(self_attention=SimpleNamespace(**sa), **et), 16, 2)
+    assert set(plain.state_dict()) == set(bare.state_dict())
+    assert not any("relative" in n or "gate" in n for n in plain.state_dict())
+    net = EpipolarTransformer(EpipolarTransformerCfg(
+        self_attention=ImageSelfAttentionCfg(**sa, relative_buckets=8, gated_mlp=True, norm_groups=4), **et,
+        refinement_groups=8), 16, 2)
+    inner = net.transformer.layers[0][1].fn.self_attention.transformer.layers[0]
+    assert isinstance(inner[1].fn, GatedFeedForward) and inner[0].fn.relative_bias.table.shape == (64, 2)
+    new = set(net.state_dict()) - set(plain.state_dict())
+    assert any(n.endswith("relative_bias.table") for n in new) and any(n.endswith("upscale_refinement.1.weight") for n in new)
+    assert FeedForward(4, 8)(torch.zeros(2, 4)).shape == (2, 4)
+    with pytest.raises(ValueError, match="self-attention"):
+        Attention(8, 2, 4, selfatt=False, kv_dim=8, relative_buckets=8)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        GatedFeedForward(8, 16)(torch.zeros(2, 8))
