@@ -34,6 +34,7 @@ struct Operand {
 struct Product {
   int m, n, k;            // n: columns of the result (forward: hidden units); k: of one half
   int halves;             // of the contraction index
+  int first;              // blockIdx.z + first: which of a's matrices, where halves is 1
   Operand a, b;
   int tiles_m, tiles_n, splits, slices_per_split;
 };
@@ -57,8 +58,8 @@ struct Copier {
   int64_t other, step;      // from the first matrix to the second; elements of a contraction index
 
   template <bool PAIRED>
-  __device__ __forceinline__ void init(const Operand& o, int row0, int rows, int wave, int lane) {
-    const T* p0 = reinterpret_cast<const T*>(o.p[0]);
+  __device__ __forceinline__ void init(const Operand& o, int which, int row0, int rows, int wave, int lane) {
+    const T* p0 = reinterpret_cast<const T*>(which ? o.p[1] : o.p[0]);
     const T* p1 = reinterpret_cast<const T*>(o.p[1]);
     other = (reinterpret_cast<const char*>(p1) - reinterpret_cast<const char*>(p0)) / (int)sizeof(T);
     step = ACROSS ? o.ld : 1;
@@ -68,7 +69,7 @@ struct Copier {
       if (ACROSS) {
         constexpr int kChunks = ROWS / kVec<T>;                  // of a row of the tile
         const int k = pos / kChunks;
-        const int row = row0 + ((pos % kChunks) ^ across_swizzle<T>(k)) * kVec<T>;
+        const int row = row0 + ((pos % kChunks) ^ across_swizzle<T, ROWS>(k)) * kVec<T>;
         at[j] = row < rows ? p0 + k * o.ld + row : nullptr;
         kk[j] = k;
       } else {
@@ -107,8 +108,8 @@ product_kernel(Product g, EP ep) {
 
   Copier<T, BM, WAVES, A_ACROSS> ca;
   Copier<T, BN, WAVES, B_ACROSS> cb;
-  ca.template init<false>(g.a, m0, g.m, wave, lane);
-  cb.template init<PAIRED>(g.b, n0, g.n, wave, lane);
+  ca.template init<false>(g.a, blockIdx.z + g.first, m0, g.m, wave, lane);
+  cb.template init<PAIRED>(g.b, 0, n0, g.n, wave, lane);
 
   floatx16 acc[TM][TN];
 #pragma unroll
@@ -124,6 +125,7 @@ product_kernel(Product g, EP ep) {
     cb.copy(which, k0, g.k, lds + buf * (kA + kB) + kA, wave);
   };
   if (s0 < s1) load(s0, 0);
+  wait_for_copies();
   __syncthreads();
   for (int s = s0; s < s1; ++s) {
     const int buf = (s - s0) & 1;
@@ -151,6 +153,7 @@ product_kernel(Product g, EP ep) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = mfma(fa[i], fb[j], acc[i][j]);
     }
+    wait_for_copies();
     __syncthreads();                                 // the next slice has arrived, this one has been read
   }
   ep.template store<T, TM, TN>(acc, m0 + wm * TM * 32, n0 + wn * TN * 32, lane, g, tm * WM + wm);
@@ -240,8 +243,8 @@ struct StoreGatedGrad {
 
 // the product itself, or this split's part of it in fp32
 struct StoreMatrix {
-  void* c;
-  float* parts;           // [splits][m][n] or NULL
+  void* c[2];             // by blockIdx.z
+  float* parts;           // [blockIdx.z][splits][m][n] or NULL
   template <typename T, int TM, int TN>
   __device__ __forceinline__ void store(const floatx16 (&acc)[TM][TN], int row0, int col0, int lane, const Product& g, int) {
 #pragma unroll
@@ -254,25 +257,14 @@ struct StoreMatrix {
         for (int r = 0; r < 16; ++r) {
           const int row = row0 + i * 32 + result_row(r, lane >> 5);
           if (row >= g.m) continue;
-          if (parts) parts[((int64_t)blockIdx.y * g.m + row) * g.n + col] = acc[i][j][r];
-          else reinterpret_cast<T*>(c)[(int64_t)row * g.n + col] = from_f32<T>(acc[i][j][r]);
+          if (parts) parts[(((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * g.m + row) * g.n + col] = acc[i][j][r];
+          else reinterpret_cast<T*>(blockIdx.z ? c[1] : c[0])[(int64_t)row * g.n + col] = from_f32<T>(acc[i][j][r]);
         }
     }
   }
 };
 
 // ---- small kernels ----------------------------------------------------------------------------------------------
-// c = sum of the parts, in their order
-template <typename T>
-__global__ void __launch_bounds__(256) join_parts_kernel(int64_t count, int splits, const float* __restrict__ parts,
-                                                         T* __restrict__ c) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= count) return;
-  float t = 0.f;
-  for (int s = 0; s < splits; ++s) t += parts[s * count + i];
-  c[i] = from_f32<T>(t);
-}
-
 // fp32: da, du of the kept projections.  A block takes `rows` rows of 256 columns and leaves their column sums.
 __global__ void __launch_bounds__(256) gated_slope_kernel(int m, int n, int ld, int rows, int act, const float* __restrict__ a,
                                                           const float* __restrict__ u, const float* __restrict__ dh,
@@ -303,22 +295,55 @@ __global__ void __launch_bounds__(256) gated_slope_kernel(int m, int n, int ld, 
   }
 }
 
-// dbg | dbu: 16 columns a block, 16 threads a column, the parts in order
+// What is left of a backward pass, in one launch: sums of the splits' parts (each in their order), and the biases'
+// gradients from the column sums of all rows' parts (16 columns a block, 16 threads a column).
+struct Join {
+  int64_t count;          // elements (a multiple of 4) of one matrix
+  int splits, matrices, blocks;
+  const float* parts;     // [matrices][splits][count]
+  void* c[2];
+};
+struct Finish {
+  Join join[2];
+  int sum_parts, hidden, ld, bias_blocks;
+  const float* sums;
+  void* db[2];
+};
 template <typename T>
-__global__ void __launch_bounds__(256) gated_bias_kernel(int parts, int n, int ld, const float* __restrict__ sums,
-                                                         T* __restrict__ dbg, T* __restrict__ dbu) {
+__global__ void __launch_bounds__(256) gated_finish_kernel(Finish f) {
   __shared__ double lds[16][17];
-  const int col = blockIdx.x * 16 + (threadIdx.x & 15), l = threadIdx.x >> 4;
+  int block = blockIdx.x;
+  for (int k = 0; k < 2; ++k) {
+    const Join& q = f.join[k];
+    if (block < q.blocks) {
+      const int64_t i = ((int64_t)block * 256 + threadIdx.x) * 4;
+      if (i >= q.count * q.matrices) return;
+      const int which = i >= q.count;
+      const float* p = q.parts + which * (q.splits - 1) * q.count + i;
+      float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int s = 0; s < q.splits; ++s) {
+        const float4 v = *reinterpret_cast<const float4*>(p + s * q.count);
+        t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
+      }
+      Pack<T, 4> out = {{from_f32<T>(t.x), from_f32<T>(t.y), from_f32<T>(t.z), from_f32<T>(t.w)}};
+      *reinterpret_cast<Pack<T, 4>*>((T*)(which ? q.c[1] : q.c[0]) + (i - which * q.count)) = out;
+      return;
+    }
+    block -= q.blocks;
+  }
+  const int col = block * 16 + (threadIdx.x & 15), l = threadIdx.x >> 4;
   double t = 0;
-  if (col < 2 * ld)
-    for (int p = l; p < parts; p += 16) t += sums[(int64_t)p * 2 * ld + col];
+  if (col < 2 * f.ld)
+#pragma unroll 4
+    for (int p = l; p < f.sum_parts; p += 16) t += f.sums[(int64_t)p * 2 * f.ld + col];
   lds[l][threadIdx.x & 15] = t;
   __syncthreads();
-  if (l == 0 && col < 2 * ld) {
+  if (l == 0 && col < 2 * f.ld) {
     for (int k = 1; k < 16; ++k) t += lds[k][threadIdx.x];
-    const int f = col < ld ? col : col - ld;
-    T* out = col < ld ? dbg : dbu;
-    if (out && f < n) out[f] = from_f32<T>((float)t);
+    const int u = col < f.ld ? col : col - f.ld;
+    T* out = (T*)(col < f.ld ? f.db[0] : f.db[1]);
+    if (out && u < f.hidden) out[u] = from_f32<T>((float)t);
   }
 }
 
@@ -379,20 +404,22 @@ constexpr int kFewRows = 8;
 
 struct Tiling { int bm, bn, splits, slices_per_split, tiles_m, tiles_n; };
 
-// columns: of the tiles (forward: 2 n).  A big tile needs two passes over the machine to pay for its tail.
-Tiling tiling(int dtype, int m, int columns, int k, int halves, bool may_split) {
+// columns: of the tiles (forward: 2 n); products: in the launch.  The largest tile that still fills the machine, twice
+// where a tile is big; a contraction is split where even small tiles do not, into 4 slices of it at least.
+Tiling tiling(int dtype, int m, int columns, int k, int halves, int products, bool may_split) {
   Tiling t;
   const int kk = kSliceBytes / (dtype == PS_DTYPE_F32 ? 4 : 2);
   auto count = [](int a, int b) { return (a + b - 1) / b; };
-  t.bm = t.bn = 128;
-  if (dtype != PS_DTYPE_F32 && (int64_t)count(m, 256) * count(columns, 256) >= 2 * kCus) t.bm = t.bn = 256;
+  auto tiles = [&](int size) { return (int64_t)count(m, size) * count(columns, size) * products; };
+  t.bm = dtype != PS_DTYPE_F32 && tiles(256) >= 2 * kCus ? 256 : tiles(128) >= kCus ? 128 : 64;
+  t.bn = t.bm;
   t.tiles_m = count(m, t.bm);
   t.tiles_n = count(columns, t.bn);
-  const int slices = count(k, kk) * halves, tiles = t.tiles_m * t.tiles_n;
+  const int slices = count(k, kk) * halves;
   t.splits = 1;
-  if (may_split && tiles < kCus) {               // fill the machine, at least 8 slices a split
-    int s = (2 * kCus) / tiles;
-    if (s > slices / 8) s = slices / 8;
+  if (may_split && tiles(t.bm) < 2 * kCus) {
+    int s = (int)(4 * kCus / tiles(t.bm));
+    if (s > slices / 4) s = slices / 4;
     t.splits = s < 1 ? 1 : s;
   }
   t.slices_per_split = count(slices, t.splits);
@@ -401,12 +428,12 @@ Tiling tiling(int dtype, int m, int columns, int k, int halves, bool may_split) 
 }
 
 template <typename T, bool A_ACROSS, bool B_ACROSS, bool PAIRED, typename EP>
-int launch_product(Product g, const Tiling& t, const EP& ep, hipStream_t st) {
+int launch_product(Product g, const Tiling& t, const EP& ep, hipStream_t st, int products = 1) {
   g.tiles_m = t.tiles_m;
   g.tiles_n = t.tiles_n;
   g.splits = t.splits;
   g.slices_per_split = t.slices_per_split;
-  const dim3 grid((unsigned)(t.tiles_m * t.tiles_n), (unsigned)t.splits);
+  const dim3 grid((unsigned)(t.tiles_m * t.tiles_n), (unsigned)t.splits, (unsigned)products);
   const size_t lds = (size_t)2 * (t.bm + t.bn) * kSliceBytes;
   if constexpr (sizeof(T) == 2) {
     if (t.bm == 256) {
@@ -418,7 +445,12 @@ int launch_product(Product g, const Tiling& t, const EP& ep, hipStream_t st) {
       return PS_OK;
     }
   }
-  product_kernel<T, 128, 128, 2, 2, A_ACROSS, B_ACROSS, PAIRED, EP><<<grid, 256, lds, st>>>(g, ep);
+  if (t.bm == 128) {
+    product_kernel<T, 128, 128, 2, 2, A_ACROSS, B_ACROSS, PAIRED, EP><<<grid, 256, lds, st>>>(g, ep);
+  } else {
+    constexpr int WN = PAIRED ? 1 : 2;               // a wave of a pair holds 32 columns of each
+    product_kernel<T, 64, 64, 2, WN, A_ACROSS, B_ACROSS, PAIRED, EP><<<grid, 128 * WN, lds, st>>>(g, ep);
+  }
   return PS_OK;
 }
 
@@ -428,26 +460,25 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 struct BackwardPlan {
   int ld, sum_parts, slope_rows;
   Tiling again, dx, dw;
-  size_t da, du, sums, parts, total;
+  size_t da, du, sums, parts_x, parts_w, total;
 };
 
 BackwardPlan backward_plan(const PsGatedLinearDesc& d) {
   BackwardPlan p;
   const size_t e = d.dtype == PS_DTYPE_F32 ? 4 : 2;
   p.ld = pad8(d.hidden);
-  p.again = tiling(d.dtype, d.rows, 2 * p.ld, d.dim, 1, false);
-  p.dx = tiling(d.dtype, d.rows, d.dim, d.hidden, 2, true);
-  p.dw = tiling(d.dtype, d.hidden, d.dim, d.rows, 1, true);
-  p.slope_rows = 32;
+  p.again = tiling(d.dtype, d.rows, 2 * p.ld, d.dim, 1, 1, false);
+  p.dx = tiling(d.dtype, d.rows, d.dim, d.hidden, 2, 1, true);
+  p.dw = tiling(d.dtype, d.hidden, d.dim, d.rows, 1, 2, true);
+  p.slope_rows = 8;
+  while (p.slope_rows < 64 && (int64_t)d.rows * p.ld > (int64_t)p.slope_rows * 256 * 8 * kCus) p.slope_rows *= 2;
   p.sum_parts = d.dtype == PS_DTYPE_F32 ? (d.rows + p.slope_rows - 1) / p.slope_rows : p.again.tiles_m * 2;
   size_t at = 0;
   p.da = at; at += align256(e * d.rows * p.ld);
   p.du = at; at += align256(e * d.rows * p.ld);
   p.sums = at; at += align256(sizeof(float) * p.sum_parts * 2 * p.ld);
-  p.parts = at;
-  const size_t px = p.dx.splits > 1 ? sizeof(float) * p.dx.splits * (size_t)d.rows * d.dim : 0;
-  const size_t pw = p.dw.splits > 1 ? sizeof(float) * p.dw.splits * (size_t)d.hidden * d.dim : 0;
-  at += align256(px > pw ? px : pw);
+  p.parts_x = at; at += p.dx.splits > 1 ? align256(sizeof(float) * p.dx.splits * (size_t)d.rows * d.dim) : 0;
+  p.parts_w = at; at += p.dw.splits > 1 ? align256(sizeof(float) * 2 * p.dw.splits * (size_t)d.hidden * d.dim) : 0;
   p.total = at;
   return p;
 }
@@ -472,14 +503,7 @@ int forward_typed(const PsGatedLinearDesc& d, const void* x, const void* wg, con
   g.a.p[0] = x; g.a.ld = d.x_row_stride;
   g.b.p[0] = wg; g.b.p[1] = wu; g.b.ld = d.w_row_stride;
   StoreGated ep = {h, bg, bu, a, u, d.activation};
-  return launch_product<T, false, false, true>(g, tiling(d.dtype, d.rows, 2 * d.hidden, d.dim, 1, false), ep, st);
-}
-
-template <typename T>
-int join(const Tiling& t, int64_t count, const float* parts, void* c, hipStream_t st) {
-  if (t.splits > 1)
-    join_parts_kernel<T><<<(unsigned)((count + 255) / 256), 256, 0, st>>>(count, t.splits, parts, (T*)c);
-  return PS_OK;
+  return launch_product<T, false, false, true>(g, tiling(d.dtype, d.rows, 2 * d.hidden, d.dim, 1, 1, false), ep, st);
 }
 
 template <typename T>
@@ -490,7 +514,9 @@ int backward_typed(const PsGatedLinearDesc& d, const void* x, const void* wg, co
   T* da = (T*)(ws + p.da);
   T* du = (T*)(ws + p.du);
   float* sums = dbg || dbu ? (float*)(ws + p.sums) : nullptr;
-  float* parts = (float*)(ws + p.parts);
+  float* parts_x = p.dx.splits > 1 ? (float*)(ws + p.parts_x) : nullptr;
+  float* parts_w = p.dw.splits > 1 ? (float*)(ws + p.parts_w) : nullptr;
+  Finish f = {};
   if constexpr (sizeof(T) == 4) {
     const dim3 grid((unsigned)((p.ld + 255) / 256), (unsigned)p.sum_parts);
     gated_slope_kernel<<<grid, 256, 0, st>>>(d.rows, d.hidden, p.ld, p.slope_rows, d.activation, a, u, (const float*)dh,
@@ -503,28 +529,34 @@ int backward_typed(const PsGatedLinearDesc& d, const void* x, const void* wg, co
     StoreGatedGrad ep = {dh, d.dh_row_stride, bg, bu, da, du, p.ld, sums, d.activation};
     if (int rc = launch_product<T, false, false, true>(g, p.again, ep, st)) return rc;
   }
-  if (sums)
-    gated_bias_kernel<T><<<(unsigned)((2 * p.ld + 15) / 16), 256, 0, st>>>(p.sum_parts, d.hidden, p.ld, sums, (T*)dbg, (T*)dbu);
+  auto join = [](const Tiling& t, int64_t count, const float* parts, int matrices, void* c0, void* c1) {
+    Join j = {count, t.splits, matrices, (int)((count * matrices / 4 + 255) / 256), parts, {c0, c1}};
+    return j;
+  };
   if (dx) {
     Product g = {};
     g.m = d.rows; g.n = d.dim; g.k = d.hidden; g.halves = 2;
     g.a.p[0] = da; g.a.p[1] = du; g.a.ld = p.ld;
     g.b.p[0] = wg; g.b.p[1] = wu; g.b.ld = d.w_row_stride;
-    StoreMatrix ep = {dx, p.dx.splits > 1 ? parts : nullptr};
+    StoreMatrix ep = {{dx, nullptr}, parts_x};
     if (int rc = launch_product<T, false, true, false>(g, p.dx, ep, st)) return rc;
-    join<T>(p.dx, (int64_t)d.rows * d.dim, parts, dx, st);
+    if (parts_x) f.join[0] = join(p.dx, (int64_t)d.rows * d.dim, parts_x, 1, dx, nullptr);
   }
-  for (int half = 0; half < 2; ++half) {
-    void* dw = half ? dwu : dwg;
-    if (!dw) continue;
+  if (dwg || dwu) {                                  // both in one launch
+    const int products = dwg && dwu ? 2 : 1;
     Product g = {};
-    g.m = d.hidden; g.n = d.dim; g.k = d.rows; g.halves = 1;
-    g.a.p[0] = half ? du : da; g.a.ld = p.ld;
+    g.m = d.hidden; g.n = d.dim; g.k = d.rows; g.halves = 1; g.first = dwg ? 0 : 1;
+    g.a.p[0] = da; g.a.p[1] = du; g.a.ld = p.ld;
     g.b.p[0] = x; g.b.ld = d.x_row_stride;
-    StoreMatrix ep = {dw, p.dw.splits > 1 ? parts : nullptr};
-    if (int rc = launch_product<T, true, true, false>(g, p.dw, ep, st)) return rc;
-    join<T>(p.dw, (int64_t)d.hidden * d.dim, parts, dw, st);
+    StoreMatrix ep = {{dwg ? dwg : dwu, dwu}, parts_w};
+    if (int rc = launch_product<T, true, true, false>(g, p.dw, ep, st, products)) return rc;
+    if (parts_w) f.join[1] = join(p.dw, (int64_t)d.hidden * d.dim, parts_w, products, dwg ? dwg : dwu, dwu);
   }
+  f.sum_parts = p.sum_parts; f.hidden = d.hidden; f.ld = p.ld; f.sums = sums;
+  f.bias_blocks = sums ? (2 * p.ld + 15) / 16 : 0;
+  f.db[0] = dbg; f.db[1] = dbu;
+  const int blocks = f.join[0].blocks + f.join[1].blocks + f.bias_blocks;
+  if (blocks) gated_finish_kernel<T><<<blocks, 256, 0, st>>>(f);
   return PS_OK;
 }
 

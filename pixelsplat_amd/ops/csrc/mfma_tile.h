@@ -48,14 +48,29 @@ __device__ __forceinline__ floatx16 zero16() {
   return z;
 }
 
-typedef __attribute__((address_space(3))) char LdsChar;
-__device__ __forceinline__ LdsChar* lds_cast(void* p) { return (LdsChar*)p; }
-
-// 16 bytes a lane from global memory to lds + 16 lane (lds is the wave's: uniform); complete after a __syncthreads
-__device__ __forceinline__ void copy_to_lds(const void* g, void* lds) {
+// Copies from global memory into LDS, 16 or 4 bytes a lane, to lds + 16 (4) lane; lds is the wave's own (uniform).
+// copy_to_lds is issued past the compiler: it would have every LDS read it cannot tell apart from a copy's target wait for all
+// copies in flight, which is the next tile's.  So a wave waits for its own with wait_for_copies, in front of the
+// barrier behind which the tile is read.  (The instruction has no result registers, and its address is read at issue.
+// M0 is a reserved register that nothing else in a kernel with these copies uses.)  For the tiled product that is 255
+// instead of 307 us (16384-long contraction of 4096 x 1024, bf16); the attention's forward, four blocks a CU and softmax
+// between its products, is slower for it (163 against 142 us) and takes copy_known.
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
+}
+__device__ __forceinline__ void copy_to_lds(const void* g, const void* lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_address(lds)), "v"(g) : "memory");
+}
+// the same as the compiler knows them (it waits by itself)
+__device__ __forceinline__ void copy_known(const void* g, void* lds) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
                                    (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
+__device__ __forceinline__ void copy_word_known(const void* g, void* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
+                                   (__attribute__((address_space(3))) void*)lds, 4, 0, 0);
+}
+__device__ __forceinline__ void wait_for_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // ---- LDS tiles ------------------------------------------------------------------------------------------------
 // Along: [rows][128 bytes of the contraction index].  The 16-byte chunk c of row r lies at c ^ ((r >> 1) & 7), so that
@@ -69,10 +84,13 @@ __device__ __forceinline__ Frag<T> along_fragment(const char* tile, int row, int
 
 // Across: [contraction index][ROWS elements].  16-bit types: the transposing LDS read hands each lane of 16 the four
 // values of one column of a 4 x 16 block; the four contraction rows of a block lie in different 64-byte parts of
-// the banks (chunk ^ 4 (k & 3)).  fp32: four 4-byte reads; the two halves of the wave read contraction indices 4
-// apart, which lie in different halves of the banks (chunk ^ 8 ((k >> 2) & 1)).
-template <typename T>
-__device__ __forceinline__ int across_swizzle(int k) { return sizeof(T) == 2 ? (k & 3) << 2 : ((k >> 2) & 1) << 3; }
+// the banks (chunk ^ 4 (k & 3); rows of 64 elements are half the banks long: chunk ^ 4 ((k >> 1) & 1)).  fp32: four
+// 4-byte reads; the two halves of the wave read contraction indices 4 apart, which lie in different halves of the banks
+// (chunk ^ 8 ((k >> 2) & 1)).
+template <typename T, int ROWS>
+__device__ __forceinline__ int across_swizzle(int k) {
+  return sizeof(T) == 4 ? ((k >> 2) & 1) << 3 : ROWS == 64 ? ((k >> 1) & 1) << 2 : (k & 3) << 2;
+}
 
 // rows `row0` .. + 31, contraction indices k0 + half * kVec .. ; k0 is a multiple of 4
 template <typename T, int ROWS>
@@ -80,7 +98,7 @@ __device__ __forceinline__ Frag<T> across_fragment(const char* tile, int row0, i
   // k0, k1: the first index of the fragment's first and second four (16-bit), or of its only four (fp32: k0)
   if constexpr (sizeof(T) == 2) {
     const int i = lane & 15, col = row0 + (lane & 16) + (i & 3) * 4, kr = i >> 2;
-    const int within = ((((col >> 3) ^ (kr << 2)) << 4) | ((col & 4) << 1));
+    const int within = ((((col >> 3) ^ across_swizzle<T, ROWS>(kr)) << 4) | ((col & 4) << 1));   // k0, k1: multiples of 4
     typedef __attribute__((address_space(3))) shortx4 lds_shortx4;
     const shortx4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4*)(tile + (k0 + kr) * (ROWS * 2) + within));
     const shortx4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4*)(tile + (k1 + kr) * (ROWS * 2) + within));
@@ -88,7 +106,7 @@ __device__ __forceinline__ Frag<T> across_fragment(const char* tile, int row0, i
     return __builtin_bit_cast(Frag<T>, v);
   } else {
     const int col = row0 + (lane & 31);
-    const int within = (((col >> 2) ^ across_swizzle<T>(k0)) << 4) | ((col & 3) << 2);
+    const int within = (((col >> 2) ^ across_swizzle<T, ROWS>(k0)) << 4) | ((col & 3) << 2);
     Frag<T> v;
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float*>(tile + (k0 + j) * (ROWS * 4) + within);

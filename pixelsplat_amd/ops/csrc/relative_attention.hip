@@ -20,10 +20,13 @@
 // fp32 too: do.o of the rounded o would put its rounding into every ds of the row.  A row's maximum and the inverse of
 // its sum are kept apart: their sum as a logarithm would lose the second where all biases of a row are at the lowest value.
 //
-// d_table without atomics on memory, in a fixed order: in the dq pass each wave adds its ds into a ring of its own in
-// LDS, indexed by code(key) + const - code(query); the 32 queries of a half wave have 32 different offsets to one key,
-// and the halves add one after the other.  What lies behind the next tile's first code is final and leaves the ring
-// for the wave's row in memory; two small kernels add the rows of all waves by offset and the offsets by bucket.
+// d_table without atomics, in a fixed order.  In a row-numbered grid the pairs of one difference key - query have just two
+// offsets: key and query in columns that ascend (key column >= query column), or that wrap.  So in the dq pass a wave
+// writes a 32 x 32 tile of ds to LDS, in rows of 65 words with 33 zeros before each, and reads it along the diagonals:
+// one difference a lane, neighbouring lanes in neighbouring banks, two sums (one where the grid is one row).  A tile's
+// 63 differences are 32 final ones and 31 that the next tile of keys adds to, which stay in registers; the final ones
+// go to the wave's row in memory.  Two small kernels add the rows by offset and the offsets by bucket.  (LDS float
+// atomics on a table of offsets measured 1487 us for the dq pass at 2 x 8 heads, 64 x 64 tokens of 64.)
 //
 // Bound by the matrix instructions in fp32, by the vector instructions of the softmax in 16 bits, by the keys' and
 // values' bytes for a few queries, which split the keys over blocks and join their partial results.
@@ -34,8 +37,11 @@ namespace ps {
 namespace {
 
 __device__ const uint4 kZeros[1] = {{0, 0, 0, 0}};
+__device__ const uint8_t kOnes[1] = {1};
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kInf = __builtin_inff();
+
+typedef int intx4 __attribute__((ext_vector_type(4)));
 
 struct Strides { int64_t b, h, t; };
 
@@ -54,14 +60,16 @@ struct Args {
   float* o32;                     // the same in fp32 or NULL
   float* stats;                   // [2][batch heads][nq_pad] or NULL: maximum (log2; +inf: no keys), 1 / sum (0: no keys)
   float *part_o, *part_ml;        // [splits][batch heads nq][dim], [..][2]
+  int join_lanes;                 // threads that share a row's splits
   // backward
   const void* dout;
   Strides sdo;
   const float* o_kept;            // fp32 o
   float* delta;                   // [batch heads][nq_pad]: do.o / sum
   void *dq, *dk, *dv;
-  float* ring_rows;               // [batch heads][nq_pad / 32][ring_pitch]
-  int ring, ring_pitch;
+  float *part_q, *part_k, *part_v;   // [splits][like dq, dk, dv] fp32, where there are splits
+  float* diag_rows;               // [batch heads][nq_pad / 32][splits of dq][1 or 2][diag_pitch]
+  int diag_pitch, diag_end;       // words of a row; differences that all splits' rows hold
 };
 
 __device__ __forceinline__ int code_of(int t, int gw) { return t + (int)((unsigned)t / (unsigned)gw) * (gw - 1); }
@@ -127,7 +135,7 @@ __device__ __forceinline__ void copy_tile(const T* base, int64_t stride, int dim
     const int pos = (j * WAVES + wave) * 64 + lane, row = pos / kChunks;
     const int d = ((pos % kChunks) ^ swizzle<PITCH>(row)) * kVec<T>;
     const bool on = ((bits >> row) & 1) && d < dim;
-    copy_to_lds(on ? (const void*)(base + (row * (int)stride + d)) : (const void*)kZeros, tile + (j * WAVES + wave) * 1024);
+    copy_known(on ? (const void*)(base + (row * (int)stride + d)) : (const void*)kZeros, tile + (j * WAVES + wave) * 1024);
   }
 }
 
@@ -136,9 +144,7 @@ template <int WAVES>
 __device__ __forceinline__ void copy_window(const float* bias, int offsets, int first, int window, float* lds, int wave,
                                             int lane) {
   for (int i = wave * 64; i < window; i += WAVES * 64)
-    __builtin_amdgcn_global_load_lds(
-        (const __attribute__((address_space(1))) void*)(bias + min(max(first + i + lane, 0), offsets - 1)),
-        (__attribute__((address_space(3))) void*)(lds + i), 4, 0, 0);
+    copy_word_known(bias + min(max(first + i + lane, 0), offsets - 1), lds + i);
 }
 
 // a lane's column operand: 16-byte chunks 2 s + hi of its row
@@ -177,10 +183,16 @@ struct Lds {                                            // bytes
   __host__ __device__ static int buffer(int window) { return kWindow + window * 4; }
 };
 
-// whether the lane's row of a tile is there
-__device__ __forceinline__ bool row_there(int first, int count, int rows, const uint8_t* mask, int lane) {
-  const int i = first + lane;
-  return lane < rows && i < count && (mask == nullptr || mask[i] != 0);
+// what the wave wrote to LDS before is what its lanes read after
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// The byte that says whether a row of a tile is there: loaded a tile ahead and without a branch, so that nothing waits for
+// it before it is used.
+__device__ __forceinline__ uint8_t mask_byte(const uint8_t* mask, int row, int count) {
+  return *(mask ? mask + min(row, count - 1) : kOnes);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -232,12 +244,12 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 128 && (sizeof(T) == 4 || WA
   const int tiles = (p.nk + ROWS - 1) / ROWS;
   const int t0 = split * p.tiles_per_split, t1 = min(t0 + p.tiles_per_split, tiles);
   uint64_t bits = 0, next_bits = 0;
-  bool there = row_there(t0 * ROWS, p.nk, ROWS, mask, lane);
+  uint8_t there = mask_byte(mask, t0 * ROWS + lane, p.nk);
   auto load = [&](int kt, int buf) {
     char* at = lds + buf * bytes;
     const int k0 = kt * ROWS;
-    next_bits = __ballot(there);                       // read a tile ahead
-    there = row_there(k0 + ROWS, p.nk, ROWS, mask, lane);
+    next_bits = __ballot(there != 0 && lane < ROWS && k0 + lane < p.nk);
+    there = mask_byte(mask, k0 + ROWS + lane, p.nk);
     copy_tile<T, PITCH, ROWS, WAVES>(kb + k0 * p.sk.t, p.sk.t, p.dim, next_bits, at, wave, lane);
     copy_tile<T, PITCH, ROWS, WAVES>(vb + k0 * p.sv.t, p.sv.t, p.dim, next_bits, at + L::kTile, wave, lane);
     int* codes = reinterpret_cast<int*>(at + 2 * L::kTile);
@@ -267,7 +279,7 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 128 && (sizeof(T) == 4 || WA
         s[u] = mfma(along<T, PITCH>(tk, u * 32 + (lane & 31), 2 * f + hi), qf[f], s[u]);
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
-        const int4 c = *reinterpret_cast<const int4*>(codes + u * 32 + 8 * a + 4 * hi);
+        const intx4 c = *reinterpret_cast<const intx4*>(codes + u * 32 + 8 * a + 4 * hi);
         s[u][4 * a + 0] = fmaf(s[u][4 * a + 0], p.scale, window[c.x]);
         s[u][4 * a + 1] = fmaf(s[u][4 * a + 1], p.scale, window[c.y]);
         s[u][4 * a + 2] = fmaf(s[u][4 * a + 2], p.scale, window[c.z]);
@@ -339,37 +351,62 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 128 && (sizeof(T) == 4 || WA
   if (p.o32) store_columns<float, DP>(o, by, p.o32 + row, p.dim, hi);
 }
 
-// the splits of a row, joined: a thread takes 4 columns
+// The splits of a row, joined.  A thread takes 4 columns and every join_lanes-th split; those of a row meet in LDS.
 template <typename T>
 __global__ void __launch_bounds__(256) join_splits_kernel(Args p) {
-  const int per = p.dim / 4;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)p.batch * p.heads * p.nq_pad;
-  const int64_t at = i / per;
-  const int d = (int)(i % per) * 4;
-  if (at >= rows) return;
+  __shared__ float lds[256][7];
+  const int per = p.dim / 4, lanes = p.join_lanes, row_threads = per * lanes, in_block = 256 / row_threads;
+  const int in = threadIdx.x % row_threads, part = in / per, d = (in % per) * 4;
+  const int64_t at = (int64_t)blockIdx.x * in_block + threadIdx.x / row_threads, rows = (int64_t)p.batch * p.heads * p.nq_pad;
   const int bh = (int)(at / p.nq_pad), qi = (int)(at % p.nq_pad);
-  if (qi >= p.nq) {
-    if (p.stats && d == 0) {
-      p.stats[at] = kInf;
-      p.stats[rows + at] = 0.f;
-    }
-    return;
-  }
+  const bool on = (int)threadIdx.x < in_block * row_threads && at < rows && qi < p.nq;
   const int64_t all = (int64_t)p.batch * p.heads * p.nq, row = (int64_t)bh * p.nq + qi;
-  float m = -kInf;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[(s * all + row) * 2]);
-  const float base = m == -kInf ? 0.f : m;
-  float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < p.splits; ++s) {
-    const float by = __builtin_amdgcn_exp2f(p.part_ml[(s * all + row) * 2] - base);
-    l = fmaf(p.part_ml[(s * all + row) * 2 + 1], by, l);
-    const float4 v = *reinterpret_cast<const float4*>(p.part_o + (s * all + row) * p.dim + d);
-    o[0] = fmaf(v.x, by, o[0]);
-    o[1] = fmaf(v.y, by, o[1]);
-    o[2] = fmaf(v.z, by, o[2]);
-    o[3] = fmaf(v.w, by, o[3]);
+  float m = -kInf, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  if (on) {
+#pragma unroll 4
+    for (int s = part; s < p.splits; s += lanes) m = fmaxf(m, p.part_ml[(s * all + row) * 2]);
+    const float base = m == -kInf ? 0.f : m;
+#pragma unroll 4
+    for (int s = part; s < p.splits; s += lanes) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * all + row) * 2);
+      const float4 v = *reinterpret_cast<const float4*>(p.part_o + (s * all + row) * p.dim + d);
+      const float by = __builtin_amdgcn_exp2f(ml.x - base);
+      l = fmaf(ml.y, by, l);
+      o[0] = fmaf(v.x, by, o[0]);
+      o[1] = fmaf(v.y, by, o[1]);
+      o[2] = fmaf(v.z, by, o[2]);
+      o[3] = fmaf(v.w, by, o[3]);
+    }
   }
-  const float by = l == 0.f ? 0.f : 1.f / l;
+  if (lanes > 1) {
+    float* mine = lds[threadIdx.x];
+    mine[0] = m;
+    mine[1] = l;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mine[2 + j] = o[j];
+    __syncthreads();
+    if (on && part == 0) {
+      float top = m;
+      for (int k = 1; k < lanes; ++k) top = fmaxf(top, lds[threadIdx.x + k * per][0]);
+      const float base = top == -kInf ? 0.f : top;
+      l = o[0] = o[1] = o[2] = o[3] = 0.f;
+      for (int k = 0; k < lanes; ++k) {
+        const float* other = lds[threadIdx.x + k * per];
+        const float by = __builtin_amdgcn_exp2f(other[0] - base);
+        l = fmaf(other[1], by, l);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = fmaf(other[2 + j], by, o[j]);
+      }
+      m = top;
+    }
+  }
+  if (part != 0 || (int)threadIdx.x >= in_block * row_threads || at >= rows) return;
+  const float by = on && l != 0.f ? 1.f / l : 0.f;
+  if (p.stats && d == 0) {
+    p.stats[at] = by != 0.f ? m : kInf;
+    p.stats[rows + at] = by;
+  }
+  if (!on) return;
   const int64_t to = (((int64_t)(bh / p.heads) * p.nq + qi) * p.heads + bh % p.heads) * p.dim + d;
   Pack<T, 4> v;
 #pragma unroll
@@ -378,21 +415,19 @@ __global__ void __launch_bounds__(256) join_splits_kernel(Args p) {
     if (p.o32) p.o32[to + j] = o[j] * by;
   }
   *reinterpret_cast<Pack<T, 4>*>((T*)p.out + to) = v;
-  if (p.stats && d == 0) {
-    p.stats[at] = l != 0.f ? m : kInf;
-    p.stats[rows + at] = by;
-  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// dq, do.o and the rings of d_table.  Columns are queries, rows are keys, as in the forward.
-template <typename T, int DP, int WAVES, bool RING>
-__global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || (RING && DP == 128) ? 1 : 2) attention_dq_kernel(Args p) {
+constexpr int kDiagRow = 65, kDiagZeros = 33, kDiag = 33 * kDiagRow + 3;      // words; of a wave: 33 rows, a multiple of 4
+
+// dq, do.o and the diagonals of ds (SUMS a difference; 0: none).  Columns are queries, rows are keys, as in the forward.
+template <typename T, int DP, int WAVES, int SUMS>
+__global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || (SUMS && DP == 128) ? 1 : 2) attention_dq_kernel(Args p) {
   constexpr int PITCH = DP * sizeof(T), ROWS = kRows<T>, SUBS = ROWS / 32, KF = DP / kFragK<T>, PF = 32 / kFragK<T>;
   typedef Lds<T, DP, WAVES> L;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, hi = lane >> 5;
-  const int tile = blockIdx.x % p.col_tiles, bh = blockIdx.x / p.col_tiles;
+  const int tile = blockIdx.x % p.col_tiles, bh = blockIdx.x / p.col_tiles, split = blockIdx.y;
   const int b = bh / p.heads, h = bh % p.heads;
   const int first = tile * WAVES * 32, last = max(min(first + WAVES * 32, p.nq) - 1, 0);
   const int qi = first + wave * 32 + (lane & 31);
@@ -423,20 +458,27 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || (RING && DP == 1
     m = p.stats[at];
     inv = p.stats[(int64_t)p.batch * p.heads * p.nq_pad + at];
     delta *= inv;
-    if (hi == 0) p.delta[at] = delta;
+    if (hi == 0 && split == 0) p.delta[at] = delta;
   }
 
-  // the wave's ring: entry u of its row is the offset u - ring_base of the head
-  float* ring = reinterpret_cast<float*>(lds + 2 * bytes) + wave * p.ring;
-  const int wave_first = min(first + wave * 32, last), wave_last = min(first + wave * 32 + 31, last);
-  const int wave_code = code_of(p.q_start + wave_last, p.gw);
-  const int ring_off = wave_code - code_of(p.q_start + min(qi, wave_last), p.gw);
-  const int q_span = wave_code - code_of(p.q_start + wave_first, p.gw);
+  // The wave's tile of ds and its row: entry i holds the difference i - 31 + (first key's token) - (first query's token).
+  const int tiles = (p.nk + ROWS - 1) / ROWS;
+  const int t0 = split * p.tiles_per_split, t1 = min(t0 + p.tiles_per_split, tiles);
   const bool wave_on = first + wave * 32 < p.nq;
-  float* ring_row = nullptr;
-  if (RING) {
-    ring_row = p.ring_rows + ((int64_t)bh * (p.nq_pad / 32) + (first / 32 + wave)) * p.ring_pitch;
-    for (int i = lane; i < p.ring; i += 64) ring[i] = 0.f;
+  float* diag = reinterpret_cast<float*>(lds + 2 * bytes) + wave * kDiag;
+  float* diag_row = nullptr;
+  int wave_col = 0, diff_col = 0, step_col = 0;         // columns: of the first query, of the lane's difference, 32 more
+  float carry[2] = {0.f, 0.f};
+  if (SUMS) {
+    diag_row = p.diag_rows + (((int64_t)bh * (p.nq_pad / 32) + (first / 32 + wave)) * p.splits + split) * SUMS * p.diag_pitch;
+    for (int i = lane; i < kDiag; i += 64) diag[i] = 0.f;
+    if (SUMS == 2) {
+      const int token = p.q_start + first + wave * 32;
+      wave_col = __builtin_amdgcn_readfirstlane((unsigned)token % (unsigned)p.gw);
+      step_col = 32 % p.gw;
+      diff_col = (t0 * ROWS + lane - 31 - token) % p.gw;
+      if (diff_col < 0) diff_col += p.gw;
+    }
   }
 
   const T* kb = (const T*)p.k + b * p.sk.b + h * p.sk.h;
@@ -447,14 +489,13 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || (RING && DP == 1
 #pragma unroll
   for (int t = 0; t < DP / 32; ++t) dq[t] = zero16();
 
-  const int tiles = (p.nk + ROWS - 1) / ROWS;
   uint64_t bits = 0, next_bits = 0;
-  bool there = row_there(0, p.nk, ROWS, mask, lane);
+  uint8_t there = mask_byte(mask, t0 * ROWS + lane, p.nk);
   auto load = [&](int kt, int buf) {
     char* at = lds + buf * bytes;
     const int k0 = kt * ROWS;
-    next_bits = __ballot(there);                       // read a tile ahead
-    there = row_there(k0 + ROWS, p.nk, ROWS, mask, lane);
+    next_bits = __ballot(there != 0 && lane < ROWS && k0 + lane < p.nk);
+    there = mask_byte(mask, k0 + ROWS + lane, p.nk);
     copy_tile<T, PITCH, ROWS, WAVES>(kb + k0 * p.sk.t, p.sk.t, p.dim, next_bits, at, wave, lane);
     copy_tile<T, PITCH, ROWS, WAVES>(vb + k0 * p.sv.t, p.sv.t, p.dim, next_bits, at + L::kTile, wave, lane);
     int* codes = reinterpret_cast<int*>(at + 2 * L::kTile);
@@ -463,17 +504,16 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || (RING && DP == 1
     copy_window<WAVES>(bias, p.offsets, c0 - code_last + p.origin, p.window,
                        reinterpret_cast<float*>(at + L::kWindow), wave, lane);
   };
-  load(0, 0);
+  load(t0, 0);
   __syncthreads();
-  for (int kt = 0; kt < tiles; ++kt) {
-    const int buf = kt & 1;
+  for (int kt = t0; kt < t1; ++kt) {
+    const int buf = (kt - t0) & 1;
     bits = next_bits;
-    if (kt + 1 < tiles) load(kt + 1, buf ^ 1);
+    if (kt + 1 < t1) load(kt + 1, buf ^ 1);
     const char* tk = lds + buf * bytes;
     const char* tv = tk + L::kTile;
     const int* codes = reinterpret_cast<const int*>(tk + 2 * L::kTile);
     const float* window = reinterpret_cast<const float*>(tk + L::kWindow) + q_off;
-    const int c0 = code_of(kt * ROWS, p.gw);
     const bool whole = bits == (ROWS == 64 ? ~0ull : 0xffffffffull);
 #pragma unroll
     for (int u = 0; u < SUBS; ++u) {
@@ -485,7 +525,7 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || (RING && DP == 1
       }
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
-        const int4 c = *reinterpret_cast<const int4*>(codes + u * 32 + 8 * a + 4 * hi);
+        const intx4 c = *reinterpret_cast<const intx4*>(codes + u * 32 + 8 * a + 4 * hi);
         const int cs[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -499,21 +539,31 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || (RING && DP == 1
         for (int r = 0; r < 16; ++r)
           if (!((mine >> (8 * (r >> 2) + (r & 3))) & 1)) ds[r] = 0.f;
       }
-      if (RING && wave_on) {
+      if (SUMS && wave_on) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (hi == half) {
+        for (int r = 0; r < 16; ++r) diag[(lane & 31) * kDiagRow + kDiagZeros + result_row(r, hi)] = ds[r];
+        wave_order();
+        float sum[2] = {0.f, 0.f};
+        int col = wave_col;
 #pragma unroll
-            for (int a = 0; a < 4; ++a) {
-              const int4 c = *reinterpret_cast<const int4*>(codes + u * 32 + 8 * a + 4 * hi);
-              const int cs[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                __hip_atomic_fetch_add(&ring[(c0 + cs[j] + ring_off) & (p.ring - 1)], ds[4 * a + j], __ATOMIC_RELAXED,
-                                       __HIP_MEMORY_SCOPE_WORKGROUP);
-            }
+        for (int i = 0; i < 32; ++i) {                  // query i of the wave, key i + lane - 31 of the tile
+          const float v = diag[i * (kDiagRow + 1) + lane + (kDiagZeros - 31)];
+          sum[0] += v;
+          if (SUMS == 2) {
+            sum[1] += col + diff_col >= p.gw ? v : 0.f;
+            col = col + 1 == p.gw ? 0 : col + 1;
           }
-          __builtin_amdgcn_wave_barrier();
+        }
+        wave_order();
+        if (SUMS == 2) {
+          sum[0] -= sum[1];
+          diff_col += step_col;
+          if (diff_col >= p.gw) diff_col -= p.gw;
+        }
+#pragma unroll
+        for (int c = 0; c < SUMS; ++c) {
+          if (lane < 32) diag_row[c * p.diag_pitch + (kt - t0) * ROWS + u * 32 + lane] = sum[c] + carry[c];
+          carry[c] = __shfl_xor(sum[c], 32);
         }
       }
 #pragma unroll
@@ -523,19 +573,20 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || (RING && DP == 1
         for (int t = 0; t < DP / 32; ++t) dq[t] = mfma(across<T, PITCH>(tk, u * 32, f, t * 32, lane), sf, dq[t]);
       }
     }
-    if (RING && wave_on) {
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      const int end = kt + 1 < tiles ? code_of((kt + 1) * ROWS, p.gw) : code_of(p.nk - 1, p.gw) + q_span + 1;
-      for (int i = c0 + lane; i < end; i += 64) {
-        ring_row[i] = ring[i & (p.ring - 1)];
-        ring[i & (p.ring - 1)] = 0.f;
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
     __syncthreads();
   }
-  if (q_on && p.dq)
-    store_columns<T, DP>(dq, p.scale * (1.f / kLog2e), (T*)p.dq + (((int64_t)b * p.nq + qi) * p.heads + h) * p.dim, p.dim, hi);
+  if (SUMS && wave_on && lane < 32) {
+#pragma unroll
+    for (int c = 0; c < SUMS; ++c) diag_row[c * p.diag_pitch + (t1 - t0) * ROWS + lane] = carry[c];
+  }
+  if (q_on && p.dq) {
+    const int64_t row = (((int64_t)b * p.nq + qi) * p.heads + h) * p.dim;
+    const float by = p.scale * (1.f / kLog2e);
+    if (p.splits > 1)
+      store_columns<float, DP>(dq, by, p.part_q + split * ((int64_t)p.batch * p.nq * p.heads * p.dim) + row, p.dim, hi);
+    else
+      store_columns<T, DP>(dq, by, (T*)p.dq + row, p.dim, hi);
+  }
 }
 
 // dk, dv.  Columns are keys, rows are queries.
@@ -545,7 +596,7 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || DP == 128 ? 1 : 
   typedef Lds<T, DP, WAVES> L;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, hi = lane >> 5;
-  const int tile = blockIdx.x % p.col_tiles, bh = blockIdx.x / p.col_tiles;
+  const int tile = blockIdx.x % p.col_tiles, bh = blockIdx.x / p.col_tiles, split = blockIdx.y;
   const int b = bh / p.heads, h = bh % p.heads;
   const int first = tile * WAVES * 32, last = min(first + WAVES * 32, p.nk) - 1;
   const int ki = first + wave * 32 + (lane & 31);
@@ -569,10 +620,11 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || DP == 128 ? 1 : 
   for (int t = 0; t < DP / 32; ++t) dk[t] = dv[t] = zero16();
 
   const int tiles = (p.nq + ROWS - 1) / ROWS;
+  const int t0 = split * p.tiles_per_split, t1 = min(t0 + p.tiles_per_split, tiles);
   auto load = [&](int qt, int buf) {
     char* at = lds + buf * bytes;
     const int q0 = qt * ROWS, end = min(q0 + ROWS, p.nq) - 1;
-    const uint64_t bits = __ballot(row_there(q0, p.nq, ROWS, nullptr, lane));
+    const uint64_t bits = __ballot(lane < ROWS && q0 + lane < p.nq);
     copy_tile<T, PITCH, ROWS, WAVES>(qb + q0 * p.sq.t, p.sq.t, p.dim, bits, at, wave, lane);
     copy_tile<T, PITCH, ROWS, WAVES>(db + q0 * p.sdo.t, p.sdo.t, p.dim, bits, at + L::kTile, wave, lane);
     // codes count down from the tile's last query, whose window entry is the first
@@ -582,17 +634,15 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || DP == 128 ? 1 : 
     if ((int)threadIdx.x < ROWS)
       codes[threadIdx.x] = c1 - code_of(p.q_start + min(q0 + (int)threadIdx.x, end), p.gw);
     for (int i = wave; i < 3; i += WAVES)                          // nq_pad holds whole tiles
-      __builtin_amdgcn_global_load_lds(
-          (const __attribute__((address_space(1))) void*)(stat_rows[i] + q0 + min(lane, ROWS - 1)),
-          (__attribute__((address_space(3))) void*)(rows + 64 * i), 4, 0, 0);
+      copy_word_known(stat_rows[i] + q0 + min(lane, ROWS - 1), rows + 64 * i);
     copy_window<WAVES>(bias, p.offsets, code_first - c1 + p.origin, p.window,
                        reinterpret_cast<float*>(at + L::kWindow), wave, lane);
   };
-  load(0, 0);
+  load(t0, 0);
   __syncthreads();
-  for (int qt = 0; qt < tiles; ++qt) {
-    const int buf = qt & 1;
-    if (qt + 1 < tiles) load(qt + 1, buf ^ 1);
+  for (int qt = t0; qt < t1; ++qt) {
+    const int buf = (qt - t0) & 1;
+    if (qt + 1 < t1) load(qt + 1, buf ^ 1);
     const char* tq = lds + buf * bytes;
     const char* td = tq + L::kTile;
     const int* codes = reinterpret_cast<const int*>(tq + 2 * L::kTile);
@@ -608,10 +658,10 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || DP == 128 ? 1 : 
       }
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
-        const int4 c = *reinterpret_cast<const int4*>(codes + u * 32 + 8 * a + 4 * hi);
-        const float4 e = *reinterpret_cast<const float4*>(rows + u * 32 + 8 * a + 4 * hi);
-        const float4 w = *reinterpret_cast<const float4*>(rows + 64 + u * 32 + 8 * a + 4 * hi);
-        const float4 g = *reinterpret_cast<const float4*>(rows + 128 + u * 32 + 8 * a + 4 * hi);
+        const intx4 c = *reinterpret_cast<const intx4*>(codes + u * 32 + 8 * a + 4 * hi);
+        const floatx4 e = *reinterpret_cast<const floatx4*>(rows + u * 32 + 8 * a + 4 * hi);
+        const floatx4 w = *reinterpret_cast<const floatx4*>(rows + 64 + u * 32 + 8 * a + 4 * hi);
+        const floatx4 g = *reinterpret_cast<const floatx4*>(rows + 128 + u * 32 + 8 * a + 4 * hi);
         const int cs[4] = {c.x, c.y, c.z, c.w};
         const float es[4] = {e.x, e.y, e.z, e.w}, ws[4] = {w.x, w.y, w.z, w.w}, gs[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
@@ -640,48 +690,110 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || DP == 128 ? 1 : 
 #pragma unroll
       for (int t = 0; t < DP / 32; ++t) dk[t] = dv[t] = zero16();
     }
-    if (p.dk) store_columns<T, DP>(dk, p.scale * (1.f / kLog2e), (T*)p.dk + row, p.dim, hi);
-    if (p.dv) store_columns<T, DP>(dv, 1.f, (T*)p.dv + row, p.dim, hi);
+    const float by = p.scale * (1.f / kLog2e);
+    const int64_t part = split * ((int64_t)p.batch * p.nk * p.heads * p.dim) + row;
+    if (p.dk && p.splits > 1) store_columns<float, DP>(dk, by, p.part_k + part, p.dim, hi);
+    else if (p.dk) store_columns<T, DP>(dk, by, (T*)p.dk + row, p.dim, hi);
+    if (p.dv && p.splits > 1) store_columns<float, DP>(dv, 1.f, p.part_v + part, p.dim, hi);
+    else if (p.dv) store_columns<T, DP>(dv, 1.f, (T*)p.dv + row, p.dim, hi);
   }
 }
 
-// d_offsets[head][o] = sum of the rings' rows: 64 offsets a block, 4 threads an offset take every 4th row
-__global__ void __launch_bounds__(256) join_rings_kernel(Args p, double* __restrict__ d_offsets) {
-  __shared__ double lds[4][64];
-  const int o = blockIdx.x * 64 + (threadIdx.x & 63), h = blockIdx.y, part = threadIdx.x >> 6;
-  const int waves = (p.nq + 31) / 32, code_end = code_of(p.nk - 1, p.gw);
+// d_offsets[head][o] = the sum of the waves' rows at the offset's difference: 16 offsets a block, 16 threads an offset take
+// every 16th row
+__global__ void __launch_bounds__(256) join_diagonals_kernel(Args p, int sums, double* __restrict__ d_offsets) {
+  __shared__ double lds[16][17];
+  const int o = blockIdx.x * 16 + (threadIdx.x & 15), h = blockIdx.y, part = threadIdx.x >> 4;
+  const int waves = (p.nq + 31) / 32, pitch = 2 * p.gw - 1, per = p.nq_pad / 32;
   double t = 0;
   if (o < p.offsets) {
-    for (int i = part; i < p.batch * waves; i += 4) {
-      const int b = i / waves, w = i % waves;
-      const int first = w * 32, last = min(first + 31, p.nq - 1);
-      const int c1 = code_of(p.q_start + last, p.gw), span = c1 - code_of(p.q_start + first, p.gw);
-      const int u = o - p.origin + c1;
-      if (u >= 0 && u <= code_end + span)
-        t += p.ring_rows[((int64_t)(b * p.heads + h) * (p.nq_pad / 32) + w) * p.ring_pitch + u];
+    const int dy = o / pitch - p.origin / pitch, dx = o % pitch - (p.gw - 1);
+    const int at = dy * p.gw + dx + 31 + p.q_start;     // at the first wave; 32 more at each next
+    const float* rows = p.diag_rows + (dx < 0 ? p.diag_pitch : 0) * (sums - 1);
+    const int len = p.diag_pitch - 32, end = p.diag_end;        // a split's keys; what the waves' rows hold
+    // the waves whose rows hold the difference
+    const int w0 = at < 0 ? (-at + 31) / 32 : 0, w1 = at >= end ? 0 : min(waves, (end - 1 - at) / 32 + 1), n = max(w1 - w0, 0);
+#pragma unroll 4
+    for (int i = part; i < p.batch * n; i += 16) {
+      const int b = i / n, w = w0 + i % n, u = at + 32 * w;
+      const int s = min(u / len, p.splits - 1), in = u - s * len;
+      const float* row = rows + (((int64_t)(b * p.heads + h) * per + w) * p.splits + s) * sums * p.diag_pitch;
+      t += row[in];
+      if (s > 0 && in < 32) t += row[in + len - (int64_t)sums * p.diag_pitch];   // the end of the split before
     }
   }
-  lds[part][threadIdx.x & 63] = t;
+  lds[part][threadIdx.x & 15] = t;
   __syncthreads();
-  if (part == 0 && o < p.offsets)
-    d_offsets[(int64_t)h * p.offsets + o] = (lds[0][threadIdx.x] + lds[1][threadIdx.x]) + (lds[2][threadIdx.x] + lds[3][threadIdx.x]);
+  if (part == 0 && o < p.offsets) {
+    for (int k = 1; k < 16; ++k) t += lds[k][threadIdx.x];
+    d_offsets[(int64_t)h * p.offsets + o] = t;
+  }
 }
 
-// d_table[bucket][head]: a wave a (bucket, head)
+// dq, dk, dv of their splits' parts, in order
+struct Parts {
+  const float* from;
+  void* to;
+  int64_t count;          // elements, a multiple of 4
+  int splits, blocks;
+};
+struct Gradients { Parts g[3]; };
+template <typename T>
+__global__ void __launch_bounds__(256) join_gradients_kernel(Gradients a) {
+  int block = blockIdx.x;
+  for (int k = 0; k < 3; ++k) {
+    const Parts& q = a.g[k];
+    if (block < q.blocks) {
+      const int64_t i = ((int64_t)block * 256 + threadIdx.x) * 4;
+      if (i >= q.count) return;
+      float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int s = 0; s < q.splits; ++s) {
+        const float4 v = *reinterpret_cast<const float4*>(q.from + s * q.count + i);
+        t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
+      }
+      Pack<T, 4> out = {{from_f32<T>(t.x), from_f32<T>(t.y), from_f32<T>(t.z), from_f32<T>(t.w)}};
+      *reinterpret_cast<Pack<T, 4>*>((T*)q.to + i) = out;
+      return;
+    }
+    block -= q.blocks;
+  }
+}
+
+constexpr int kJoinHeads = 8;
+
+// d_table[bucket][head]: a block a bucket and 8 heads; every block reads the map, 8 entries a thread at a time
 template <typename T>
 __global__ void __launch_bounds__(256) join_offsets_kernel(int heads, int offsets, int buckets, const int32_t* __restrict__ map,
                                                            const double* __restrict__ d_offsets, void* __restrict__ d_table,
                                                            int table_f32) {
-  const int bucket = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (bucket >= buckets) return;
-  for (int h = blockIdx.y; h < heads; h += gridDim.y) {
-    double t = 0;
-    for (int o = lane; o < offsets; o += 64)
-      if (map[o] == bucket) t += d_offsets[(int64_t)h * offsets + o];
+  __shared__ double lds[4][kJoinHeads];
+  const int bucket = blockIdx.x, lane = threadIdx.x & 63, h0 = blockIdx.y * kJoinHeads;
+  double t[kJoinHeads];
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) t += __shfl_xor(t, m);
-    if (lane == 0) store_param<T>(d_table, table_f32, (int64_t)bucket * heads + h, (float)t);
+  for (int j = 0; j < kJoinHeads; ++j) t[j] = 0;
+  for (int base = threadIdx.x; base < offsets; base += 256 * 8) {
+    int mine[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mine[i] = base + i * 256 < offsets ? map[base + i * 256] : -1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (mine[i] == bucket) {
+#pragma unroll
+        for (int j = 0; j < kJoinHeads; ++j)
+          if (h0 + j < heads) t[j] += d_offsets[(int64_t)(h0 + j) * offsets + base + i * 256];
+      }
   }
+#pragma unroll
+  for (int j = 0; j < kJoinHeads; ++j) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) t[j] += __shfl_xor(t[j], m);
+    if (lane == 0) lds[threadIdx.x >> 6][j] = t[j];
+  }
+  __syncthreads();
+  const int j = threadIdx.x;
+  if (j < kJoinHeads && h0 + j < heads)
+    store_param<T>(d_table, table_f32, (int64_t)bucket * heads + h0 + j, (float)((lds[0][j] + lds[1][j]) + (lds[2][j] + lds[3][j])));
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -696,10 +808,22 @@ int span_of(int n, int gh, int gw) {
   return (n - 1) + crossings * (gw - 1);
 }
 
+struct Split { int splits, tiles; };     // tiles of each
+
+// few blocks: split the streamed side, `least` tiles a split at least
+Split split_of(int64_t blocks, int want, int tiles, int least) {
+  int s = blocks < want ? (int)(want / blocks) : 1;
+  if (s > tiles / least) s = tiles / least;
+  if (s < 1) s = 1;
+  const int per = count(tiles, s);
+  return {count(tiles, per), per};
+}
+
 struct Plan {
-  int waves, rows, tiles, splits, tiles_per_split, nq_pad, window, ring, ring_pitch, offsets, dp;
+  int waves, rows, nq_pad, window, window_b, sums, diag_pitch, offsets, dp;
+  Split forward, dq, dkv;
   size_t part_o, part_ml, forward_total;
-  size_t delta, ring_rows, d_offsets, backward_total;
+  size_t delta, diag_rows, d_offsets, part_q, part_k, part_v, backward_total;
 };
 
 Plan plan(const PsRelativeAttentionDesc& d, bool training) {
@@ -710,36 +834,39 @@ Plan plan(const PsRelativeAttentionDesc& d, bool training) {
   p.offsets = (2 * d.grid_h - 1) * (2 * d.grid_w - 1);
   p.nq_pad = count(d.queries, 64) * 64;
   p.waves = d.queries <= 32 ? 1 : 4;
-  p.tiles = count(nk, p.rows);
-  const int64_t blocks = (int64_t)d.batch * d.heads * count(training ? p.nq_pad : d.queries, p.waves * 32);
-  // few blocks: split the keys, at least 4 tiles a split (a join reads and writes a row of o per split)
-  const int want = p.waves == 1 ? 1536 : 512;
-  p.splits = 1;
-  if (blocks < want / 2) {
-    int s = (int)(want / blocks);
-    if (s > p.tiles / 4) s = p.tiles / 4;
-    p.splits = s < 1 ? 1 : s;
-  }
-  p.tiles_per_split = count(p.tiles, p.splits);
-  p.splits = count(p.tiles, p.tiles_per_split);
-  const int cols = 128;      // at most
-  const int wide = span_of(cols, d.grid_h, d.grid_w) + span_of(p.rows, d.grid_h, d.grid_w) + 1;
-  p.window = count(wide, 64) * 64;
-  const int live = span_of(32, d.grid_h, d.grid_w) + span_of(p.rows, d.grid_h, d.grid_w) + 1;
-  p.ring = 64;
-  while (p.ring < live) p.ring *= 2;
-  p.ring_pitch = count((nk - 1) + (int64_t)(d.grid_h - 1) * (d.grid_w - 1) + span_of(32, d.grid_h, d.grid_w) + 1, 64) * 64;
-  const size_t rows = (size_t)d.batch * d.heads * d.queries;
+  auto window = [&](int columns) {
+    return count(span_of(columns, d.grid_h, d.grid_w) + span_of(p.rows, d.grid_h, d.grid_w) + 1, 64) * 64;
+  };
+  p.window = window(p.waves * 32);
+  p.window_b = window(128);
+  const int64_t bh = (int64_t)d.batch * d.heads;
+  const int tiles = count(nk, p.rows), q_tiles = count(d.queries, p.rows);
+  // One wave a block: as many blocks as are resident at once (their LDS decides), in one round.  Four waves: two a CU.
+  const int resident = 160 * 1024 / (2 * (2 * p.rows * p.dp * e + 4 * 256 + 4 * p.window));
+  const int64_t blocks = bh * count(training ? p.nq_pad : d.queries, p.waves * 32);
+  p.forward = p.waves == 1 ? split_of(blocks, 256 * (resident < 1 ? 1 : resident > 8 ? 8 : resident), tiles, 2)
+                           : split_of(blocks, 512, tiles, 2);
+  p.dq = split_of(bh * count(p.nq_pad, 128), 512, tiles, 2);
+  p.dkv = split_of(bh * count(nk, 128), 512, q_tiles, 2);
+  p.sums = d.grid_h == 1 ? 1 : 2;
+  p.diag_pitch = p.dq.tiles * p.rows + 32;
+  const size_t rows = (size_t)bh * d.queries;
   size_t at = 0;
-  if (p.splits > 1) {
-    p.part_o = at; at += align256(sizeof(float) * p.splits * rows * d.dim);
-    p.part_ml = at; at += align256(sizeof(float) * p.splits * rows * 2);
+  auto take = [&](size_t bytes) { const size_t here = at; at += align256(bytes); return here; };
+  if (p.forward.splits > 1) {
+    p.part_o = take(sizeof(float) * p.forward.splits * rows * d.dim);
+    p.part_ml = take(sizeof(float) * p.forward.splits * rows * 2);
   }
   p.forward_total = at + 256;
   at = 0;
-  p.delta = at; at += align256(sizeof(float) * d.batch * d.heads * p.nq_pad);
-  p.ring_rows = at; at += align256(sizeof(float) * d.batch * d.heads * (p.nq_pad / 32) * p.ring_pitch);
-  p.d_offsets = at; at += align256(sizeof(double) * d.heads * p.offsets);
+  p.delta = take(sizeof(float) * bh * p.nq_pad);
+  p.diag_rows = take(sizeof(float) * bh * (p.nq_pad / 32) * p.dq.splits * p.sums * p.diag_pitch);
+  p.d_offsets = take(sizeof(double) * d.heads * p.offsets);
+  if (p.dq.splits > 1) p.part_q = take(sizeof(float) * p.dq.splits * rows * d.dim);
+  if (p.dkv.splits > 1) {
+    p.part_k = take(sizeof(float) * p.dkv.splits * bh * nk * d.dim);
+    p.part_v = take(sizeof(float) * p.dkv.splits * bh * nk * d.dim);
+  }
   p.backward_total = at + 256;
   return p;
 }
@@ -753,8 +880,8 @@ Args args_of(const PsRelativeAttentionDesc& d, const Plan& p) {
   a.mask_b = d.mask_stride;
   a.batch = d.batch; a.heads = d.heads; a.nq = d.queries; a.nk = d.grid_h * d.grid_w; a.dim = d.dim;
   a.gw = d.grid_w; a.origin = (d.grid_h - 1) * (2 * d.grid_w - 1) + d.grid_w - 1; a.offsets = p.offsets;
-  a.q_start = d.query_start; a.nq_pad = p.nq_pad; a.scale = d.scale * kLog2e; a.window = p.window;
-  a.ring = p.ring; a.ring_pitch = p.ring_pitch;
+  a.q_start = d.query_start; a.nq_pad = p.nq_pad; a.scale = d.scale * kLog2e;
+  a.diag_pitch = p.diag_pitch; a.diag_end = count(a.nk, p.rows) * p.rows + 32;
   return a;
 }
 
@@ -767,15 +894,17 @@ bool allow_lds(K kernel, size_t bytes) {
 template <typename T, int DP, int WAVES>
 int run_forward(Args a, const Plan& p, hipStream_t st) {
   a.col_tiles = count(a.stats ? a.nq_pad : a.nq, WAVES * 32);
-  a.splits = p.splits;
-  a.tiles_per_split = p.tiles_per_split;
+  a.splits = p.forward.splits;
+  a.tiles_per_split = p.forward.tiles;
+  a.window = p.window;
   const size_t lds = 2 * (size_t)Lds<T, DP, WAVES>::buffer(p.window);
   auto kernel = attention_forward_kernel<T, DP, WAVES>;
   if (!allow_lds(kernel, lds)) return PS_ERR_LAUNCH;
   kernel<<<dim3((unsigned)(a.col_tiles * a.batch * a.heads), (unsigned)a.splits), WAVES * 64, lds, st>>>(a);
   if (a.splits > 1) {
-    const int64_t items = (int64_t)a.batch * a.heads * a.nq_pad * (a.dim / 4);
-    join_splits_kernel<T><<<(unsigned)((items + 255) / 256), 256, 0, st>>>(a);
+    a.join_lanes = a.splits >= 8 ? 8 : 1;                // dim <= 128: a row's threads fit a block
+    const int in_block = 256 / (a.dim / 4 * a.join_lanes);
+    join_splits_kernel<T><<<(unsigned)(((int64_t)a.batch * a.heads * a.nq_pad + in_block - 1) / in_block), 256, 0, st>>>(a);
   }
   return PS_OK;
 }
@@ -783,25 +912,42 @@ int run_forward(Args a, const Plan& p, hipStream_t st) {
 template <typename T, int DP>
 int run_backward(Args a, const Plan& p, bool table, hipStream_t st) {
   constexpr int WAVES = 4;
-  const size_t lds = 2 * (size_t)Lds<T, DP, WAVES>::buffer(p.window);
+  const size_t lds = 2 * (size_t)Lds<T, DP, WAVES>::buffer(p.window_b);
+  a.window = p.window_b;
   const unsigned bh = (unsigned)(a.batch * a.heads);
   a.col_tiles = count(a.nq_pad, WAVES * 32);
-  if (table) {
-    const size_t with = lds + (size_t)WAVES * p.ring * 4;
-    auto kernel = attention_dq_kernel<T, DP, WAVES, true>;
-    if (!allow_lds(kernel, with)) return PS_ERR_LAUNCH;
-    kernel<<<a.col_tiles * bh, WAVES * 64, with, st>>>(a);
-  } else {
-    auto kernel = attention_dq_kernel<T, DP, WAVES, false>;
-    if (!allow_lds(kernel, lds)) return PS_ERR_LAUNCH;
-    kernel<<<a.col_tiles * bh, WAVES * 64, lds, st>>>(a);
-  }
+  a.splits = p.dq.splits;
+  a.tiles_per_split = p.dq.tiles;
+  auto dq = [&](auto kernel, size_t bytes) {
+    if (!allow_lds(kernel, bytes)) return false;
+    kernel<<<dim3(a.col_tiles * bh, (unsigned)a.splits), WAVES * 64, bytes, st>>>(a);
+    return true;
+  };
+  const size_t with = lds + (size_t)WAVES * kDiag * sizeof(float);
+  const bool ok = !table ? dq(attention_dq_kernel<T, DP, WAVES, 0>, lds)
+                  : p.sums == 1 ? dq(attention_dq_kernel<T, DP, WAVES, 1>, with)
+                                : dq(attention_dq_kernel<T, DP, WAVES, 2>, with);
+  if (!ok) return PS_ERR_LAUNCH;
   if (a.dk || a.dv) {
     a.col_tiles = count(a.nk, WAVES * 32);
+    a.splits = p.dkv.splits;
+    a.tiles_per_split = p.dkv.tiles;
     auto kernel = attention_dkv_kernel<T, DP, WAVES>;
     if (!allow_lds(kernel, lds)) return PS_ERR_LAUNCH;
-    kernel<<<a.col_tiles * bh, WAVES * 64, lds, st>>>(a);
+    kernel<<<dim3(a.col_tiles * bh, (unsigned)a.splits), WAVES * 64, lds, st>>>(a);
   }
+  Gradients g = {};
+  unsigned blocks = 0;
+  auto add = [&](int i, void* to, const float* from, int tokens, int splits) {
+    const int64_t n = (int64_t)bh * tokens * a.dim;
+    if (!to || splits <= 1) return;
+    g.g[i] = {from, to, n, splits, count(n, 1024)};
+    blocks += g.g[i].blocks;
+  };
+  add(0, a.dq, a.part_q, a.nq, p.dq.splits);
+  add(1, a.dk, a.part_k, a.nk, p.dkv.splits);
+  add(2, a.dv, a.part_v, a.nk, p.dkv.splits);
+  if (blocks) join_gradients_kernel<T><<<blocks, 256, 0, st>>>(g);
   return PS_OK;
 }
 
@@ -824,8 +970,9 @@ int backward_typed(const PsRelativeAttentionDesc& d, Args a, const Plan& p, cons
                : p.dp == 64 ? run_backward<T, 64>(a, p, d_table != nullptr, st)
                             : run_backward<T, 128>(a, p, d_table != nullptr, st);
   if (rc || !d_table) return rc;
-  join_rings_kernel<<<dim3((unsigned)count(p.offsets, 64), (unsigned)d.heads), 256, 0, st>>>(a, d_offsets);
-  join_offsets_kernel<T><<<dim3((unsigned)count(d.buckets, 4), (unsigned)d.heads), 256, 0, st>>>(
+  a.splits = p.dq.splits;
+  join_diagonals_kernel<<<dim3((unsigned)count(p.offsets, 16), (unsigned)d.heads), 256, 0, st>>>(a, p.sums, d_offsets);
+  join_offsets_kernel<T><<<dim3((unsigned)d.buckets, (unsigned)count(d.heads, kJoinHeads)), 256, 0, st>>>(
       d.heads, p.offsets, d.buckets, map, d_offsets, d_table, d.table_f32);
   return PS_OK;
 }
@@ -917,7 +1064,8 @@ int ps_relative_attention_backward(const PsRelativeAttentionDesc* d, const void*
   char* ws = (char*)workspace;
   a.q = q; a.k = k; a.v = v; a.mask = key_mask; a.bias = bias; a.dout = d_out;
   a.o_kept = out_f32; a.stats = const_cast<float*>(stats); a.delta = (float*)(ws + p.delta);
-  a.ring_rows = (float*)(ws + p.ring_rows);
+  a.diag_rows = (float*)(ws + p.diag_rows);
+  a.part_q = (float*)(ws + p.part_q); a.part_k = (float*)(ws + p.part_k); a.part_v = (float*)(ws + p.part_v);
   a.dq = dq; a.dk = dk; a.dv = dv;
   double* d_offsets = (double*)(ws + p.d_offsets);
   hipStream_t st = (hipStream_t)stream;
