@@ -50,30 +50,56 @@ __device__ __forceinline__ float sigmoid_f32(float z) { return 1.f / (1.f + __ex
 // the PS_ACT_ values of pixelsplat_ops.h
 enum Act { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_SIGMOID = 4 };
 
-template <bool EXACT>
-__device__ __forceinline__ float act_value(int act, float z) {
-  switch (act) {
-    case ACT_RELU: return z > 0.f || z != z ? z : 0.f;
-    case ACT_SILU: return z * sigmoid_f32(z);
-    case ACT_GELU: { float cdf, bell; normal_cdf<EXACT>(z, cdf, bell); return z * cdf; }
-    case ACT_SIGMOID: return sigmoid_f32(z);
-    default: return z;
+template <int ACT, bool EXACT>
+__device__ __forceinline__ float act_value(float z) {
+  if constexpr (ACT == ACT_RELU) return z > 0.f || z != z ? z : 0.f;
+  if constexpr (ACT == ACT_SILU) return z * sigmoid_f32(z);
+  if constexpr (ACT == ACT_GELU) {
+    float cdf, bell;
+    normal_cdf<EXACT>(z, cdf, bell);
+    return z * cdf;
   }
+  if constexpr (ACT == ACT_SIGMOID) return sigmoid_f32(z);
+  return z;
 }
 // act'(z); *value = act(z)
-template <bool EXACT>
-__device__ __forceinline__ float act_slope(int act, float z, float* value) {
+template <int ACT, bool EXACT>
+__device__ __forceinline__ float act_slope(float z, float* value) {
+  if constexpr (ACT == ACT_RELU) {
+    *value = z > 0.f || z != z ? z : 0.f;
+    return z > 0.f ? 1.f : 0.f;
+  }
+  if constexpr (ACT == ACT_SILU) {
+    const float s = sigmoid_f32(z);
+    *value = z * s;
+    return s * fmaf(z, 1.f - s, 1.f);
+  }
+  if constexpr (ACT == ACT_GELU) {
+    float cdf, bell;
+    normal_cdf<EXACT>(z, cdf, bell);
+    *value = z * cdf;
+    return fmaf(z * 0.39894228040143268f, bell, cdf);
+  }
+  if constexpr (ACT == ACT_SIGMOID) {
+    const float s = sigmoid_f32(z);
+    *value = s;
+    return s * (1.f - s);
+  }
+  *value = z;
+  return 1.f;
+}
+
+template <int A> struct ActTag { static constexpr int act = A; };
+// f(ActTag<act>()): one branch around a kernel's loop, whose body then holds one activation's instructions.  (A branch
+// an element left 16 - 28 KB of code in an epilogue, and the instruction cache's misses were most of a small call.)
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F f) {
   switch (act) {
-    case ACT_RELU: *value = z > 0.f || z != z ? z : 0.f; return z > 0.f ? 1.f : 0.f;
-    case ACT_SILU: { const float s = sigmoid_f32(z); *value = z * s; return s * fmaf(z, 1.f - s, 1.f); }
-    case ACT_GELU: {
-      float cdf, bell;
-      normal_cdf<EXACT>(z, cdf, bell);
-      *value = z * cdf;
-      return fmaf(z * 0.39894228040143268f, bell, cdf);
-    }
-    case ACT_SIGMOID: { const float s = sigmoid_f32(z); *value = s; return s * (1.f - s); }
-    default: *value = z; return 1.f;
+    case ACT_RELU: f(ActTag<ACT_RELU>()); break;
+    case ACT_SILU: f(ActTag<ACT_SILU>()); break;
+    case ACT_GELU: f(ActTag<ACT_GELU>()); break;
+    case ACT_SIGMOID: f(ActTag<ACT_SIGMOID>()); break;
+    default: f(ActTag<ACT_NONE>()); break;
   }
 }
 

@@ -168,6 +168,10 @@ struct StoreGated {
   int act;
   template <typename T, int TM, int TN>
   __device__ __forceinline__ void store(const floatx16 (&acc)[TM][TN], int row0, int col0, int lane, const Product& g, int) {
+    with_act(act, [&](auto tag) { run<decltype(tag)::act, T, TM, TN>(acc, row0, col0, lane, g); });
+  }
+  template <int ACT, typename T, int TM, int TN>
+  __device__ __forceinline__ void run(const floatx16 (&acc)[TM][TN], int row0, int col0, int lane, const Product& g) {
 #pragma unroll
     for (int j = 0; j < TN; j += 2) {
       const int f = (col0 + j * 32) / 2 + (lane & 31);
@@ -182,7 +186,7 @@ struct StoreGated {
           if (row >= g.m) continue;
           const float za = acc[i][j][r] + wg, zu = acc[i][j + 1][r] + wu;
           const int64_t at = (int64_t)row * g.n + f;
-          reinterpret_cast<T*>(h)[at] = from_f32<T>(act_value<sizeof(T) == 4>(act, za) * zu);
+          reinterpret_cast<T*>(h)[at] = from_f32<T>(act_value<ACT, sizeof(T) == 4>(za) * zu);
           if (a) { a[at] = za; u[at] = zu; }
         }
     }
@@ -201,6 +205,11 @@ struct StoreGatedGrad {
   template <typename T, int TM, int TN>
   __device__ __forceinline__ void store(const floatx16 (&acc)[TM][TN], int row0, int col0, int lane, const Product& g,
                                         int row_part) {
+    with_act(act, [&](auto tag) { run<decltype(tag)::act, T, TM, TN>(acc, row0, col0, lane, g, row_part); });
+  }
+  template <int ACT, typename T, int TM, int TN>
+  __device__ __forceinline__ void run(const floatx16 (&acc)[TM][TN], int row0, int col0, int lane, const Product& g,
+                                      int row_part) {
 #pragma unroll
     for (int j = 0; j < TN; j += 2) {
       const int f = (col0 + j * 32) / 2 + (lane & 31);
@@ -219,7 +228,7 @@ struct StoreGatedGrad {
           if (on) {
             const float d = to_f32(reinterpret_cast<const T*>(dh)[row * ld_dh + f]);
             float value;
-            const float slope = act_slope<sizeof(T) == 4>(act, acc[i][j][r] + wg, &value);
+            const float slope = act_slope<ACT, sizeof(T) == 4>(acc[i][j][r] + wg, &value);
             va = d * (acc[i][j + 1][r] + wu) * slope;
             vu = d * value;
           }
@@ -273,22 +282,32 @@ __global__ void __launch_bounds__(256) gated_slope_kernel(int m, int n, int ld, 
   const int f = blockIdx.x * 256 + threadIdx.x;
   if (f >= ld) return;
   const int r0 = blockIdx.y * rows, r1 = min(r0 + rows, m);
+  const int fc = min(f, n - 1);                      // the columns behind the last are zero
+  const bool on = f < n;
   float sa = 0.f, su = 0.f;
-#pragma unroll 4
-  for (int r = r0; r < r1; ++r) {
-    float va = 0.f, vu = 0.f;
-    if (f < n) {
-      const float d = dh[r * ld_dh + f];
-      float value;
-      const float slope = act_slope<true>(act, a[(int64_t)r * n + f], &value);
-      va = d * u[(int64_t)r * n + f] * slope;
-      vu = d * value;
+  with_act(act, [&](auto tag) {
+    for (int r = r0; r < r1; r += 4) {
+      float za[4], zu[4], d[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t row = min(r + i, m - 1);
+        za[i] = a[row * n + fc];
+        zu[i] = u[row * n + fc];
+        d[i] = dh[row * ld_dh + fc];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (r + i >= r1) continue;
+        float value;
+        const float slope = act_slope<decltype(tag)::act, true>(za[i], &value);
+        const float va = on ? d[i] * zu[i] * slope : 0.f, vu = on ? d[i] * value : 0.f;
+        da[(int64_t)(r + i) * ld + f] = va;
+        du[(int64_t)(r + i) * ld + f] = vu;
+        sa += va;
+        su += vu;
+      }
     }
-    da[(int64_t)r * ld + f] = va;
-    du[(int64_t)r * ld + f] = vu;
-    sa += va;
-    su += vu;
-  }
+  });
   if (sums) {
     sums[((int64_t)blockIdx.y * 2 + 0) * ld + f] = sa;
     sums[((int64_t)blockIdx.y * 2 + 1) * ld + f] = su;
@@ -391,7 +410,7 @@ __global__ void __launch_bounds__(256) gated_rows_kernel(int m, int d, int n, in
       if (i < m) {
         const float za = sa[i] + b0, zu = su[i] + b1;
         const int64_t at = (int64_t)i * n + f;
-        h[at] = from_f32<T>(act_value<sizeof(T) == 4>(act, za) * zu);
+        with_act(act, [&](auto tag) { h[at] = from_f32<T>(act_value<decltype(tag)::act, sizeof(T) == 4>(za) * zu); });
         if (a) { a[at] = za; u[at] = zu; }
       }
     }

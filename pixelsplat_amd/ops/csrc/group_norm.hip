@@ -98,22 +98,24 @@ __global__ void __launch_bounds__(1024) group_norm_held_forward_kernel(
     mean_out[blockIdx.x] = mean;
     rstd_out[blockIdx.x] = rstd;
   }
+  with_act(sh.act, [&](auto tag) {
 #pragma unroll
-  for (int j = 0; j < HELD; ++j) {
-    const int i = threadIdx.x + j * blockDim.x;
-    if (i < count) {
-      const int ch = (i % per_row) * V;
-      Pack<T, V> out;
+    for (int j = 0; j < HELD; ++j) {
+      const int i = threadIdx.x + j * blockDim.x;
+      if (i < count) {
+        const int ch = (i % per_row) * V;
+        Pack<T, V> out;
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const int c = g * sh.cg + ch + e;
-        const float ga = gamma ? load_param<T>(gamma, sh.param_f32, c) : 1.f;
-        const float be = beta ? load_param<T>(beta, sh.param_f32, c) : 0.f;
-        out.v[e] = from_f32<T>(act_value<exact_act<T>()>(sh.act, fmaf((to_f32(held[j].v[e]) - mean) * rstd, ga, be)));
+        for (int e = 0; e < V; ++e) {
+          const int c = g * sh.cg + ch + e;
+          const float ga = gamma ? load_param<T>(gamma, sh.param_f32, c) : 1.f;
+          const float be = beta ? load_param<T>(beta, sh.param_f32, c) : 0.f;
+          out.v[e] = from_f32<T>(act_value<decltype(tag)::act, exact_act<T>()>(fmaf((to_f32(held[j].v[e]) - mean) * rstd, ga, be)));
+        }
+        *reinterpret_cast<Pack<T, V>*>(yg + (int64_t)(i / per_row) * sh.c + ch) = out;
       }
-      *reinterpret_cast<Pack<T, V>*>(yg + (int64_t)(i / per_row) * sh.c + ch) = out;
     }
-  }
+  });
 }
 
 // blockDim.x is a multiple of the vectors per row: a thread's channels are the same in all its rows.
@@ -149,20 +151,22 @@ __global__ void __launch_bounds__(1024) group_norm_held_backward_kernel(
     sb[e] = sg[e] = 0.f;
   }
   float dz[HELD][V];
+  with_act(sh.act, [&](auto tag) {
 #pragma unroll
-  for (int j = 0; j < HELD; ++j) {
-    if ((int)(threadIdx.x + j * blockDim.x) < count) {
+    for (int j = 0; j < HELD; ++j) {
+      if ((int)(threadIdx.x + j * blockDim.x) < count) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float xh = (to_f32(hx[j].v[e]) - mean) * rstd;
-        float value;
-        const float d = to_f32(hd[j].v[e]) * act_slope<exact_act<T>()>(sh.act, fmaf(xh, ga[e], be[e]), &value);
-        dz[j][e] = d;
-        sb[e] += d;
-        sg[e] = fmaf(d, xh, sg[e]);
+        for (int e = 0; e < V; ++e) {
+          const float xh = (to_f32(hx[j].v[e]) - mean) * rstd;
+          float value;
+          const float d = to_f32(hd[j].v[e]) * act_slope<decltype(tag)::act, exact_act<T>()>(fmaf(xh, ga[e], be[e]), &value);
+          dz[j][e] = d;
+          sb[e] += d;
+          sg[e] = fmaf(d, xh, sg[e]);
+        }
       }
     }
-  }
+  });
   double2 sum = make_double2(0, 0);
 #pragma unroll
   for (int e = 0; e < V; ++e) {
@@ -247,14 +251,21 @@ __global__ void __launch_bounds__(kThreads) group_norm_sums_kernel(Shape sh, int
     lds[c] = t;
   }
   __syncthreads();
-  const int lane = threadIdx.x & 63;
+  // a group's channels to as many lanes, up to a wave's
+  int lanes = 1;
+  while (lanes < sh.cg && lanes < 64) lanes *= 2;
+  const int l = threadIdx.x & (lanes - 1), at_once = kThreads / lanes;
   double2* out = sums + ((int64_t)n * gridDim.x * gridDim.z + blockIdx.x * gridDim.z + blockIdx.z) * sh.groups;
-  for (int g = threadIdx.x >> 6; g < sh.groups; g += kThreads / 64) {
+  for (int g0 = 0; g0 < sh.groups; g0 += at_once) {
+    const int g = g0 + threadIdx.x / lanes;
     const int a = max(g * sh.cg - q.c0, 0), b = min((g + 1) * sh.cg - q.c0, q.nc);
     double2 t = make_double2(0, 0);
-    for (int c = a + lane; c < b; c += 64) t = t + lds[c];
-    t = wave_sum(t);
-    if (lane == 0) out[g] = t;
+    for (int c = a + l; c < b; c += lanes) t = t + lds[c];
+    for (int m = lanes >> 1; m >= 1; m >>= 1) {
+      t.x += __shfl_xor(t.x, m);
+      t.y += __shfl_xor(t.y, m);
+    }
+    if (l == 0 && g < sh.groups) out[g] = t;
   }
 }
 
@@ -266,6 +277,7 @@ __device__ __forceinline__ void fold_moments(const Shape& sh, int parts, const d
     const int g = threadIdx.x % ng, l = threadIdx.x / ng;
     double2 t = make_double2(0, 0);
     if (l < lanes)
+#pragma unroll 4
       for (int p = l; p < parts; p += lanes) t = t + sums[(int64_t)p * sh.groups + g0 + g];
     scratch[threadIdx.x] = t;
     __syncthreads();
@@ -308,15 +320,17 @@ __global__ void __launch_bounds__(kThreads) group_norm_apply_kernel(
   }
   const T* p = x + n * rx.sample + q.c0 + q.vec;
   T* o = y + (int64_t)n * sh.s * sh.c + q.c0 + q.vec;
+  with_act(sh.act, [&](auto tag) {
 #pragma unroll 4
-  for (int r = r0 + q.row0; r < r1; r += q.tr) {
-    const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(p + r * rx.row);
-    Pack<T, V> out;
+    for (int r = r0 + q.row0; r < r1; r += q.tr) {
+      const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(p + r * rx.row);
+      Pack<T, V> out;
 #pragma unroll
-    for (int e = 0; e < V; ++e)
-      out.v[e] = from_f32<T>(act_value<exact_act<T>()>(sh.act, fmaf(to_f32(v.v[e]) - mean[e], scale[e], be[e])));
-    *reinterpret_cast<Pack<T, V>*>(o + (int64_t)r * sh.c) = out;
-  }
+      for (int e = 0; e < V; ++e)
+        out.v[e] = from_f32<T>(act_value<decltype(tag)::act, exact_act<T>()>(fmaf(to_f32(v.v[e]) - mean[e], scale[e], be[e])));
+      *reinterpret_cast<Pack<T, V>*>(o + (int64_t)r * sh.c) = out;
+    }
+  });
 }
 
 // partial: [n][chunks][2][c] (sum dz | sum dz xh)
@@ -341,19 +355,21 @@ __global__ void __launch_bounds__(kThreads) group_norm_grad_sums_kernel(
     }
     const T* p = x + n * rx.sample + q.c0 + q.vec;
     const T* d = dy + n * rdy.sample + q.c0 + q.vec;
+    with_act(sh.act, [&](auto tag) {
 #pragma unroll 2
-    for (int r = r0 + q.row0; r < r1; r += q.tr) {
-      const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(p + r * rx.row);
-      const Pack<T, V> u = *reinterpret_cast<const Pack<T, V>*>(d + r * rdy.row);
+      for (int r = r0 + q.row0; r < r1; r += q.tr) {
+        const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(p + r * rx.row);
+        const Pack<T, V> u = *reinterpret_cast<const Pack<T, V>*>(d + r * rdy.row);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float xh = (to_f32(v.v[e]) - mean[e]) * rstd[e];
-        float value;
-        const float dz = to_f32(u.v[e]) * act_slope<exact_act<T>()>(sh.act, fmaf(xh, ga[e], be[e]), &value);
-        sb[e] += dz;
-        sg[e] = fmaf(dz, xh, sg[e]);
+        for (int e = 0; e < V; ++e) {
+          const float xh = (to_f32(v.v[e]) - mean[e]) * rstd[e];
+          float value;
+          const float dz = to_f32(u.v[e]) * act_slope<decltype(tag)::act, exact_act<T>()>(fmaf(xh, ga[e], be[e]), &value);
+          sb[e] += dz;
+          sg[e] = fmaf(dz, xh, sg[e]);
+        }
       }
-    }
+    });
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       lds[0][q.row0 * q.nc + q.vec + e] = sb[e];
@@ -386,6 +402,7 @@ __global__ void __launch_bounds__(kThreads) group_norm_fold_kernel(
     const float* p = partial + (int64_t)n * chunks * 2 * sh.c;
     double2 t = make_double2(0, 0);
     const int items = chunks * sh.cg;
+#pragma unroll 4
     for (int j = lane; j < items; j += 64) {
       const int chunk = j / sh.cg, c = c0 + j % sh.cg;
       const double ga = gamma ? load_param<T>(gamma, sh.param_f32, c) : 1.f;
@@ -400,6 +417,7 @@ __global__ void __launch_bounds__(kThreads) group_norm_fold_kernel(
   const int col = (blockIdx.x - group_blocks) * 16 + (threadIdx.x & 15), l = threadIdx.x >> 4;
   double t = 0;
   if (col < 2 * sh.c)
+#pragma unroll 8
     for (int64_t p = l; p < (int64_t)sh.n * chunks; p += 16) t += partial[p * 2 * sh.c + col];
   lds[l][threadIdx.x & 15] = t;
   __syncthreads();
@@ -433,20 +451,22 @@ __global__ void __launch_bounds__(kThreads) group_norm_grad_apply_kernel(
   const T* p = x + n * rx.sample + q.c0 + q.vec;
   const T* d = dy + n * rdy.sample + q.c0 + q.vec;
   T* o = dx + (int64_t)n * sh.s * sh.c + q.c0 + q.vec;
+  with_act(sh.act, [&](auto tag) {
 #pragma unroll 2
-  for (int r = r0 + q.row0; r < r1; r += q.tr) {
-    const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(p + r * rx.row);
-    const Pack<T, V> u = *reinterpret_cast<const Pack<T, V>*>(d + r * rdy.row);
-    Pack<T, V> out;
+    for (int r = r0 + q.row0; r < r1; r += q.tr) {
+      const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(p + r * rx.row);
+      const Pack<T, V> u = *reinterpret_cast<const Pack<T, V>*>(d + r * rdy.row);
+      Pack<T, V> out;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float xh = (to_f32(v.v[e]) - mean[e]) * rstd[e];
-      float value;
-      const float dz = to_f32(u.v[e]) * act_slope<exact_act<T>()>(sh.act, fmaf(xh, ga[e], be[e]), &value);
-      out.v[e] = from_f32<T>(rstd[e] * (fmaf(dz, ga[e], -m1[e]) - xh * m2[e]));
+      for (int e = 0; e < V; ++e) {
+        const float xh = (to_f32(v.v[e]) - mean[e]) * rstd[e];
+        float value;
+        const float dz = to_f32(u.v[e]) * act_slope<decltype(tag)::act, exact_act<T>()>(fmaf(xh, ga[e], be[e]), &value);
+        out.v[e] = from_f32<T>(rstd[e] * (fmaf(dz, ga[e], -m1[e]) - xh * m2[e]));
+      }
+      *reinterpret_cast<Pack<T, V>*>(o + (int64_t)r * sh.c) = out;
     }
-    *reinterpret_cast<Pack<T, V>*>(o + (int64_t)r * sh.c) = out;
-  }
+  });
 }
 
 // ---------------------------------------------------------------------------------------------------------------

@@ -841,13 +841,15 @@ Plan plan(const PsRelativeAttentionDesc& d, bool training) {
   p.window_b = window(128);
   const int64_t bh = (int64_t)d.batch * d.heads;
   const int tiles = count(nk, p.rows), q_tiles = count(d.queries, p.rows);
-  // One wave a block: as many blocks as are resident at once (their LDS decides), in one round.  Four waves: two a CU.
+  // As many blocks as are resident at once, in one round: of one wave, their LDS decides; of four, their registers (one
+  // block a CU for rows of 512 bytes, else two are enough to fill the vector pipes).
+  const int fill = p.dp * e == 512 ? 256 : 512;
   const int resident = 160 * 1024 / (2 * (2 * p.rows * p.dp * e + 4 * 256 + 4 * p.window));
   const int64_t blocks = bh * count(training ? p.nq_pad : d.queries, p.waves * 32);
   p.forward = p.waves == 1 ? split_of(blocks, 256 * (resident < 1 ? 1 : resident > 8 ? 8 : resident), tiles, 2)
-                           : split_of(blocks, 512, tiles, 2);
-  p.dq = split_of(bh * count(p.nq_pad, 128), 512, tiles, 2);
-  p.dkv = split_of(bh * count(nk, 128), 512, q_tiles, 2);
+                           : split_of(blocks, fill, tiles, 2);
+  p.dq = split_of(bh * count(p.nq_pad, 128), fill, tiles, 2);
+  p.dkv = split_of(bh * count(nk, 128), fill, q_tiles, 2);
   p.sums = d.grid_h == 1 ? 1 : 2;
   p.diag_pitch = p.dq.tiles * p.rows + 32;
   const size_t rows = (size_t)bh * d.queries;
