@@ -25,6 +25,7 @@ namespace {
 __device__ const uint4 kZeros[1] = {{0, 0, 0, 0}};   // what a copy reads for a chunk outside its operand
 
 constexpr int kSliceBytes = 128;
+typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 
 struct Operand {
   const void* p[2];       // two matrices: the halves of the contraction (dx), or of the columns (forward)
@@ -91,7 +92,40 @@ struct Copier {
   }
 };
 
-// BM x BN tile of WM x WN waves; EP(acc, row, column of the wave's tile) writes the result
+// A 16-bit tile on its way from result registers to memory: a register's 32 lanes are 64 bytes of a row, memory wants
+// 16 bytes a lane.  Rows are 16 bytes longer than they are, so that the halves of a wave, 4 rows apart, differ in banks.
+template <typename T, int ROWS, int COLS, int THREADS>
+struct Staged {
+  static constexpr int kPitch = COLS * 2 + 16, kBytes = ROWS * kPitch, kChunks = ROWS * COLS / 8 / THREADS;
+  static __device__ __forceinline__ T* at(char* tile, int row, int col) { return reinterpret_cast<T*>(tile + row * kPitch) + col; }
+  // f(chunk of the thread, row, first column)
+  template <typename F>
+  static __device__ __forceinline__ void each(F f) {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int pos = i * THREADS + threadIdx.x;
+      f(i, pos / (COLS / 8), pos % (COLS / 8) * 8);
+    }
+  }
+  // rows of out from (row0, col0): rows and columns (a multiple of 8) that there are
+  static __device__ __forceinline__ void flush(char* tile, T* out, int64_t ld, int row0, int rows, int col0, int cols) {
+    each([&](int, int row, int col) {
+      if (row0 + row < rows && col0 + col < cols)
+        *reinterpret_cast<uintx4*>(out + (row0 + row) * ld + col0 + col) = *reinterpret_cast<uintx4*>(at(tile, row, col));
+    });
+  }
+};
+
+// what an epilogue knows of its block
+template <typename T_, int BM_, int BN_, int WM_, int WN_>
+struct Tile {
+  typedef T_ T;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, THREADS = WM * WN * 64, TM = BM / WM / 32, TN = BN / WN / 32;
+  char* lds;
+  int m0, n0, wm, wn, lane, row_part;
+};
+
+// BM x BN tile of WM x WN waves; EP writes the result
 template <typename T, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, bool PAIRED, typename EP>
 __global__ void __launch_bounds__(WM * WN * 64, 2)
 product_kernel(Product g, EP ep) {
@@ -106,6 +140,7 @@ product_kernel(Product g, EP ep) {
   const int tm = group * 8 + in % rows_in, tn = in / rows_in;
   const int m0 = tm * BM, n0 = tn * BN;
 
+  const Tile<T, BM, BN, WM, WN> tile = {lds, m0, n0, wm, wn, lane, tm * WM + wm};
   Copier<T, BM, WAVES, A_ACROSS> ca;
   Copier<T, BN, WAVES, B_ACROSS> cb;
   ca.template init<false>(g.a, blockIdx.z + g.first, m0, g.m, wave, lane);
@@ -156,7 +191,7 @@ product_kernel(Product g, EP ep) {
     wait_for_copies();
     __syncthreads();                                 // the next slice has arrived, this one has been read
   }
-  ep.template store<T, TM, TN>(acc, m0 + wm * TM * 32, n0 + wn * TN * 32, lane, g, tm * WM + wm);
+  ep.store(acc, tile, g);                      // LDS is free
 }
 
 // ---- epilogues --------------------------------------------------------------------------------------------------
@@ -166,87 +201,110 @@ struct StoreGated {
   const void *bg, *bu;
   float *a, *u;           // NULL: not kept
   int act;
-  template <typename T, int TM, int TN>
-  __device__ __forceinline__ void store(const floatx16 (&acc)[TM][TN], int row0, int col0, int lane, const Product& g, int) {
-    with_act(act, [&](auto tag) { run<decltype(tag)::act, T, TM, TN>(acc, row0, col0, lane, g); });
-  }
-  template <int ACT, typename T, int TM, int TN>
-  __device__ __forceinline__ void run(const floatx16 (&acc)[TM][TN], int row0, int col0, int lane, const Product& g) {
+  template <typename TL>
+  __device__ __forceinline__ void store(const floatx16 (&acc)[TL::TM][TL::TN], const TL& t, const Product& g) const {
+    typedef typename TL::T T;
+    typedef Staged<T, TL::BM, TL::BN / 2, TL::THREADS> St;
+    const bool staged = sizeof(T) == 2 && g.n % 8 == 0;
+    const int u0 = t.n0 / 2;
+    with_act(act, [&](auto tag) {
 #pragma unroll
-    for (int j = 0; j < TN; j += 2) {
-      const int f = (col0 + j * 32) / 2 + (lane & 31);
-      if (f >= g.n) continue;
-      const float wg = bg ? to_f32(reinterpret_cast<const T*>(bg)[f]) : 0.f;
-      const float wu = bu ? to_f32(reinterpret_cast<const T*>(bu)[f]) : 0.f;
+      for (int j = 0; j < TL::TN; j += 2) {
+        const int col = (t.wn * TL::TN + j) * 16 + (t.lane & 31), f = u0 + col;
+        if (f >= g.n) continue;
+        const float wg = bg ? to_f32(reinterpret_cast<const T*>(bg)[f]) : 0.f;
+        const float wu = bu ? to_f32(reinterpret_cast<const T*>(bu)[f]) : 0.f;
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TL::TM; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int row = row0 + i * 32 + result_row(r, lane >> 5);
-          if (row >= g.m) continue;
-          const float za = acc[i][j][r] + wg, zu = acc[i][j + 1][r] + wu;
-          const int64_t at = (int64_t)row * g.n + f;
-          reinterpret_cast<T*>(h)[at] = from_f32<T>(act_value<ACT, sizeof(T) == 4>(za) * zu);
-          if (a) { a[at] = za; u[at] = zu; }
-        }
+          for (int r = 0; r < 16; ++r) {
+            const int in = (t.wm * TL::TM + i) * 32 + result_row(r, t.lane >> 5), row = t.m0 + in;
+            const float za = acc[i][j][r] + wg, zu = acc[i][j + 1][r] + wu;
+            const T v = from_f32<T>(act_value<decltype(tag)::act, sizeof(T) == 4>(za) * zu);
+            if (staged) {
+              *St::at(t.lds, in, col) = v;
+            } else if (row < g.m) {
+              const int64_t at = (int64_t)row * g.n + f;
+              reinterpret_cast<T*>(h)[at] = v;
+              if (a) { a[at] = za; u[at] = zu; }
+            }
+          }
+      }
+    });
+    if (staged) {
+      __syncthreads();
+      if constexpr (sizeof(T) == 2) St::flush(t.lds, (T*)h, g.n, t.m0, g.m, u0, g.n);
     }
   }
 };
 
-// da and du from the recomputed projections; with biases, their column sums over the wave's rows
+// da and du (16-bit) from the recomputed projections; with biases, their column sums over the wave's rows.  dh comes
+// through LDS where it lies in whole aligned chunks; da takes its place there.
 struct StoreGatedGrad {
   const void* dh;
   int64_t ld_dh;
+  int dh_chunks;          // rows of dh are whole 16-byte chunks
   const void *bg, *bu;
   void *da, *du;          // [m][ld]
   int ld;
   float* sums;            // [row parts][2][ld] or NULL
   int act;
-  template <typename T, int TM, int TN>
-  __device__ __forceinline__ void store(const floatx16 (&acc)[TM][TN], int row0, int col0, int lane, const Product& g,
-                                        int row_part) {
-    with_act(act, [&](auto tag) { run<decltype(tag)::act, T, TM, TN>(acc, row0, col0, lane, g, row_part); });
-  }
-  template <int ACT, typename T, int TM, int TN>
-  __device__ __forceinline__ void run(const floatx16 (&acc)[TM][TN], int row0, int col0, int lane, const Product& g,
-                                      int row_part) {
+  template <typename TL>
+  __device__ __forceinline__ void store(const floatx16 (&acc)[TL::TM][TL::TN], const TL& t, const Product& g) const {
+    typedef typename TL::T T;
+    typedef Staged<T, TL::BM, TL::BN / 2, TL::THREADS> St;
+    char *ta = t.lds, *tu = t.lds + St::kBytes;
+    const int u0 = t.n0 / 2;
+    if (dh_chunks) {
+      uintx4 v[St::kChunks];
+      St::each([&](int i, int row, int col) {
+        const bool there = t.m0 + row < g.m && u0 + col < g.n;
+        v[i] = *reinterpret_cast<const uintx4*>(there ? (const void*)((const T*)dh + (t.m0 + row) * ld_dh + u0 + col)
+                                                      : (const void*)kZeros);
+      });
+      St::each([&](int i, int row, int col) { *reinterpret_cast<uintx4*>(St::at(ta, row, col)) = v[i]; });
+      __syncthreads();
+    }
+    with_act(act, [&](auto tag) {
 #pragma unroll
-    for (int j = 0; j < TN; j += 2) {
-      const int f = (col0 + j * 32) / 2 + (lane & 31);
-      if (f >= ld) continue;
-      const bool on = f < g.n;                          // the columns behind the last are zero
-      const float wg = on && bg ? to_f32(reinterpret_cast<const T*>(bg)[f]) : 0.f;
-      const float wu = on && bu ? to_f32(reinterpret_cast<const T*>(bu)[f]) : 0.f;
-      float sa = 0.f, su = 0.f;
+      for (int j = 0; j < TL::TN; j += 2) {
+        const int col = (t.wn * TL::TN + j) * 16 + (t.lane & 31), f = u0 + col;
+        if (f >= ld) continue;
+        const bool on = f < g.n;                        // the columns behind the last are zero
+        const float wg = on && bg ? to_f32(reinterpret_cast<const T*>(bg)[f]) : 0.f;
+        const float wu = on && bu ? to_f32(reinterpret_cast<const T*>(bu)[f]) : 0.f;
+        float sa = 0.f, su = 0.f;
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TL::TM; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int row = row0 + i * 32 + result_row(r, lane >> 5);
-          if (row >= g.m) continue;
-          float va = 0.f, vu = 0.f;
-          if (on) {
-            const float d = to_f32(reinterpret_cast<const T*>(dh)[row * ld_dh + f]);
-            float value;
-            const float slope = act_slope<ACT, sizeof(T) == 4>(acc[i][j][r] + wg, &value);
-            va = d * (acc[i][j + 1][r] + wu) * slope;
-            vu = d * value;
+          for (int r = 0; r < 16; ++r) {
+            const int in = (t.wm * TL::TM + i) * 32 + result_row(r, t.lane >> 5), row = t.m0 + in;
+            float va = 0.f, vu = 0.f;
+            if (on && row < g.m) {
+              const float d = to_f32(dh_chunks ? *St::at(ta, in, col) : reinterpret_cast<const T*>(dh)[row * ld_dh + f]);
+              float value;
+              const float slope = act_slope<decltype(tag)::act, false>(acc[i][j][r] + wg, &value);
+              va = d * (acc[i][j + 1][r] + wu) * slope;
+              vu = d * value;
+            }
+            *St::at(ta, in, col) = from_f32<T>(va);
+            *St::at(tu, in, col) = from_f32<T>(vu);
+            sa += va;
+            su += vu;
           }
-          const int64_t at = (int64_t)row * ld + f;
-          reinterpret_cast<T*>(da)[at] = from_f32<T>(va);
-          reinterpret_cast<T*>(du)[at] = from_f32<T>(vu);
-          sa += va;
-          su += vu;
-        }
-      if (sums) {
-        sa += __shfl_xor(sa, 32);
-        su += __shfl_xor(su, 32);
-        if (lane < 32) {
-          sums[((int64_t)row_part * 2 + 0) * ld + f] = sa;
-          sums[((int64_t)row_part * 2 + 1) * ld + f] = su;
+        if (sums) {
+          sa += __shfl_xor(sa, 32);
+          su += __shfl_xor(su, 32);
+          if (t.lane < 32) {
+            sums[((int64_t)t.row_part * 2 + 0) * ld + f] = sa;
+            sums[((int64_t)t.row_part * 2 + 1) * ld + f] = su;
+          }
         }
       }
-    }
+    });
+    __syncthreads();
+    St::flush(ta, (T*)da, ld, t.m0, g.m, u0, ld);
+    St::flush(tu, (T*)du, ld, t.m0, g.m, u0, ld);
   }
 };
 
@@ -254,21 +312,29 @@ struct StoreGatedGrad {
 struct StoreMatrix {
   void* c[2];             // by blockIdx.z
   float* parts;           // [blockIdx.z][splits][m][n] or NULL
-  template <typename T, int TM, int TN>
-  __device__ __forceinline__ void store(const floatx16 (&acc)[TM][TN], int row0, int col0, int lane, const Product& g, int) {
+  template <typename TL>
+  __device__ __forceinline__ void store(const floatx16 (&acc)[TL::TM][TL::TN], const TL& t, const Product& g) const {
+    typedef typename TL::T T;
+    typedef Staged<T, TL::BM, TL::BN, TL::THREADS> St;
+    T* out = reinterpret_cast<T*>(blockIdx.z ? c[1] : c[0]);
+    const bool staged = sizeof(T) == 2 && !parts;       // n is a multiple of 8
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int col = col0 + j * 32 + (lane & 31);
+    for (int j = 0; j < TL::TN; ++j) {
+      const int in_col = (t.wn * TL::TN + j) * 32 + (t.lane & 31), col = t.n0 + in_col;
       if (col >= g.n) continue;
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+      for (int i = 0; i < TL::TM; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int row = row0 + i * 32 + result_row(r, lane >> 5);
-          if (row >= g.m) continue;
-          if (parts) parts[(((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * g.m + row) * g.n + col] = acc[i][j][r];
-          else reinterpret_cast<T*>(blockIdx.z ? c[1] : c[0])[(int64_t)row * g.n + col] = from_f32<T>(acc[i][j][r]);
+          const int in = (t.wm * TL::TM + i) * 32 + result_row(r, t.lane >> 5), row = t.m0 + in;
+          if (staged) *St::at(t.lds, in, in_col) = from_f32<T>(acc[i][j][r]);
+          else if (row < g.m && parts) parts[(((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * g.m + row) * g.n + col] = acc[i][j][r];
+          else if (row < g.m) out[(int64_t)row * g.n + col] = from_f32<T>(acc[i][j][r]);
         }
+    }
+    if (staged) {
+      __syncthreads();
+      if constexpr (sizeof(T) == 2) St::flush(t.lds, out, g.n, t.m0, g.m, t.n0, g.n);
     }
   }
 };
@@ -430,7 +496,7 @@ Tiling tiling(int dtype, int m, int columns, int k, int halves, int products, bo
   const int kk = kSliceBytes / (dtype == PS_DTYPE_F32 ? 4 : 2);
   auto count = [](int a, int b) { return (a + b - 1) / b; };
   auto tiles = [&](int size) { return (int64_t)count(m, size) * count(columns, size) * products; };
-  t.bm = dtype != PS_DTYPE_F32 && tiles(256) >= 2 * kCus ? 256 : tiles(128) >= kCus ? 128 : 64;
+    t.bm = dtype != PS_DTYPE_F32 && tiles(256) >= 2 * kCus ? 256 : tiles(128) >= kCus ? 128 : 64;
   t.bn = t.bm;
   t.tiles_m = count(m, t.bm);
   t.tiles_n = count(columns, t.bn);
@@ -453,7 +519,9 @@ int launch_product(Product g, const Tiling& t, const EP& ep, hipStream_t st, int
   g.splits = t.splits;
   g.slices_per_split = t.slices_per_split;
   const dim3 grid((unsigned)(t.tiles_m * t.tiles_n), (unsigned)t.splits, (unsigned)products);
-  const size_t lds = (size_t)2 * (t.bm + t.bn) * kSliceBytes;
+  // two buffers of slices; then at most two staged tiles of half the columns, or one of all
+  const size_t slices = (size_t)2 * (t.bm + t.bn) * kSliceBytes, staged = (size_t)t.bm * (2 * t.bn + 32);
+  const size_t lds = sizeof(T) == 2 && staged > slices ? staged : slices;
   if constexpr (sizeof(T) == 2) {
     if (t.bm == 256) {
       auto kernel = product_kernel<T, 256, 256, 2, 4, A_ACROSS, B_ACROSS, PAIRED, EP>;
@@ -545,7 +613,8 @@ int backward_typed(const PsGatedLinearDesc& d, const void* x, const void* wg, co
     g.m = d.rows; g.n = d.hidden; g.k = d.dim; g.halves = 1;
     g.a.p[0] = x; g.a.ld = d.x_row_stride;
     g.b.p[0] = wg; g.b.p[1] = wu; g.b.ld = d.w_row_stride;
-    StoreGatedGrad ep = {dh, d.dh_row_stride, bg, bu, da, du, p.ld, sums, d.activation};
+    const int chunks = d.hidden % 8 == 0 && d.dh_row_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(dh) & 15) == 0;
+    StoreGatedGrad ep = {dh, d.dh_row_stride, chunks, bg, bu, da, du, p.ld, sums, d.activation};
     if (int rc = launch_product<T, false, false, true>(g, p.again, ep, st)) return rc;
   }
   auto join = [](const Tiling& t, int64_t count, const float* parts, int matrices, void* c0, void* c1) {
@@ -605,7 +674,7 @@ extern "C" {
 int ps_gated_linear_forward(const PsGatedLinearDesc* d, const void* x, const void* w_gate, const void* w_up,
                             const void* b_gate, const void* b_up, void* h, float* gate, float* up, void* stream) {
   if (int rc = check(d, x, w_gate, w_up)) return rc;
-  if (!h || (gate == nullptr) != (up == nullptr)) return PS_ERR_BAD_ARG;
+  if (!h || !aligned16(h) || (gate == nullptr) != (up == nullptr)) return PS_ERR_BAD_ARG;
   hipStream_t st = (hipStream_t)stream;
   int rc;
   switch (d->dtype) {
@@ -628,6 +697,7 @@ int ps_gated_linear_backward(const PsGatedLinearDesc* d, const void* x, const vo
   if (int rc = check(d, x, w_gate, w_up)) return rc;
   if (!dh || !workspace || !aligned16(workspace) || d->dh_row_stride < d->hidden) return PS_ERR_BAD_ARG;
   if (d->dtype == PS_DTYPE_F32 && (!gate || !up)) return PS_ERR_BAD_ARG;
+  if (!aligned16(dx) || !aligned16(dw_gate) || !aligned16(dw_up)) return PS_ERR_BAD_ARG;
   if (workspace_bytes < backward_plan(*d).total) return PS_ERR_WORKSPACE;
   hipStream_t st = (hipStream_t)stream;
   char* ws = (char*)workspace;

@@ -55,7 +55,8 @@ int ps_group_norm_backward(const PsGroupNormDesc* desc, const void* x, const voi
  * matrices are 16-byte aligned (else PS_ERR_BAD_ARG); hidden is any number.  No projection is written to memory,
  * except gate, up [rows][hidden] fp32 (the projections with their biases) where they are not NULL: fp32 training
  * hands them to the backward, 16-bit types compute them again and take NULL there.
- * Backward: every output may be NULL.  dx [rows][dim], dw [hidden][dim], db [hidden], contiguous. */
+ * Backward: every output may be NULL.  dx [rows][dim], dw [hidden][dim], db [hidden], contiguous.  h, dx and dw are
+ * 16-byte aligned. */
 typedef struct PsGatedLinearDesc {
   int32_t rows, dim, hidden;
   int32_t dtype, activation;
