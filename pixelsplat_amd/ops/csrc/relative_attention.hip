@@ -23,7 +23,8 @@
 // d_table without atomics, in a fixed order.  In a row-numbered grid the pairs of one difference key - query have just two
 // offsets: key and query in columns that ascend (key column >= query column), or that wrap.  So in the dq pass a wave
 // writes a 32 x 32 tile of ds to LDS, in rows of 65 words with 33 zeros before each, and reads it along the diagonals:
-// one difference a lane, neighbouring lanes in neighbouring banks, two sums (one where the grid is one row).  A tile's
+// one difference a lane, neighbouring lanes in neighbouring banks, two sums; one where the tile's keys and queries each lie
+// in one row of the grid, where a difference is one offset.  A tile's
 // 63 differences are 32 final ones and 31 that the next tile of keys adds to, which stay in registers; the final ones
 // go to the wave's row in memory.  Two small kernels add the rows by offset and the offsets by bucket.  (LDS float
 // atomics on a table of offsets measured 1487 us for the dq pass at 2 x 8 heads, 64 x 64 tokens of 64.)
@@ -58,7 +59,7 @@ struct Args {
   // forward
   void* out;                      // [batch][nq][heads][dim]
   float* o32;                     // the same in fp32 or NULL
-  float* stats;                   // [2][batch heads][nq_pad] or NULL: maximum (log2; +inf: no keys), 1 / sum (0: no keys)
+  float* stats;                   // [2][batch heads][nq_pad] or NULL: maximum (log2, or up to 8 less; +inf: no keys), 1 / sum (0)
   float *part_o, *part_ml;        // [splits][batch heads nq][dim], [..][2]
   int join_lanes;                 // threads that share a row's splits
   // backward
@@ -73,6 +74,11 @@ struct Args {
 };
 
 __device__ __forceinline__ int code_of(int t, int gw) { return t + (int)((unsigned)t / (unsigned)gw) * (gw - 1); }
+
+// whether the tokens first .. first + n - 1 all exist and lie in one row of the grid
+__device__ __forceinline__ bool in_a_row(int first, int n, int tokens, int gw) {
+  return first + n <= tokens && (int)((unsigned)first % (unsigned)gw) + n <= gw;
+}
 
 template <typename T> constexpr int kRows = sizeof(T) == 2 ? 64 : 32;   // rows of a streamed tile
 
@@ -154,6 +160,39 @@ __device__ __forceinline__ void load_columns(Frag<T> (&f)[DP / kFragK<T>], const
   for (int s = 0; s < DP / kFragK<T>; ++s) {
     const int d = (2 * s + hi) * kVec<T>;
     f[s] = *reinterpret_cast<const Frag<T>*>(on && d < dim ? (const void*)(row + d) : (const void*)kZeros);
+  }
+}
+
+// Order of a product's LDS reads and matrix instructions in fp32: reads run AHEAD of them.  Left alone, the compiler puts
+// each read in front of its use and waits for it, 64 cycles of matrix work at a time (forward 38 -> 34 us, dq 62 -> 57
+// at 14 x 4 heads of 256 tokens of 128).
+template <int READS, int PRODUCTS, int AHEAD>
+__device__ __forceinline__ void reads_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < READS - AHEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS / READS, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS - (READS - AHEAD) * (PRODUCTS / READS), 0);
+}
+
+// s = s scale + bias for 32 rows.  codes: the rows' distances in the window; `line`: they are consecutive, `base` is the
+// first row's entry and `step` + or - 1 (addresses are then the lane's and a constant: an instruction an element less).
+template <int STEP>
+__device__ __forceinline__ void add_bias(floatx16& s, float scale, const float* window, const int* codes, bool line,
+                                         const float* base, int u, int hi) {
+  if (line) {
+    const float* from = base + STEP * 4 * hi;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], scale, from[STEP * (u * 32 + 8 * (r >> 2) + (r & 3))]);
+  } else {
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const intx4 c = *reinterpret_cast<const intx4*>(codes + u * 32 + 8 * a + 4 * hi);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[4 * a + j] = fmaf(s[4 * a + j], scale, window[c[j]]);
+    }
   }
 }
 
@@ -277,15 +316,11 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 128 && (sizeof(T) == 4 || WA
 #pragma unroll
       for (int f = 0; f < KF; ++f)
         s[u] = mfma(along<T, PITCH>(tk, u * 32 + (lane & 31), 2 * f + hi), qf[f], s[u]);
-#pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const intx4 c = *reinterpret_cast<const intx4*>(codes + u * 32 + 8 * a + 4 * hi);
-        s[u][4 * a + 0] = fmaf(s[u][4 * a + 0], p.scale, window[c.x]);
-        s[u][4 * a + 1] = fmaf(s[u][4 * a + 1], p.scale, window[c.y]);
-        s[u][4 * a + 2] = fmaf(s[u][4 * a + 2], p.scale, window[c.z]);
-        s[u][4 * a + 3] = fmaf(s[u][4 * a + 3], p.scale, window[c.w]);
-      }
+      if (sizeof(T) == 4) reads_ahead<KF, 4 * KF, 4>();
     }
+    const bool line = in_a_row(kt * ROWS, ROWS, p.nk, p.gw);
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u) add_bias<1>(s[u], p.scale, window, codes, line, window, u, hi);
     if (bits != (ROWS == 64 ? ~0ull : 0xffffffffull)) {
 #pragma unroll
       for (int u = 0; u < SUBS; ++u) {
@@ -300,7 +335,8 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 128 && (sizeof(T) == 4 || WA
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
     top = fmaxf(top, __shfl_xor(top, 32));
-    if (__any(top > m)) {                              // a new maximum: what there is shrinks
+    // A new maximum: what there is shrinks.  Not for every one: terms of up to 2^8 are as exact as those of up to 1.
+    if (__any(top > m + 8.f)) {
       const float nm = fmaxf(m, top);
       const float by = __builtin_amdgcn_exp2f(m - (nm == -kInf ? 0.f : nm));
       m = nm;
@@ -326,6 +362,7 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 128 && (sizeof(T) == 4 || WA
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t) o[t] = mfma(across<T, PITCH>(tv, u * 32, f, t * 32, lane), pf, o[t]);
       }
+    if (sizeof(T) == 4) reads_ahead<4 * PF * (DP / 32), 4 * PF * (DP / 32), 8>();
     __syncthreads();
   }
   l += __shfl_xor(l, 32);
@@ -467,6 +504,7 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || (SUMS && DP == 1
   const bool wave_on = first + wave * 32 < p.nq;
   float* diag = reinterpret_cast<float*>(lds + 2 * bytes) + wave * kDiag;
   float* diag_row = nullptr;
+  bool wave_line = false;                               // the wave's queries lie in one row of the grid
   int wave_col = 0, diff_col = 0, step_col = 0;         // columns: of the first query, of the lane's difference, 32 more
   float carry[2] = {0.f, 0.f};
   if (SUMS) {
@@ -475,6 +513,7 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || (SUMS && DP == 1
     if (SUMS == 2) {
       const int token = p.q_start + first + wave * 32;
       wave_col = __builtin_amdgcn_readfirstlane((unsigned)token % (unsigned)p.gw);
+      wave_line = wave_col + 32 <= p.gw;
       step_col = 32 % p.gw;
       diff_col = (t0 * ROWS + lane - 31 - token) % p.gw;
       if (diff_col < 0) diff_col += p.gw;
@@ -515,6 +554,7 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || (SUMS && DP == 1
     const int* codes = reinterpret_cast<const int*>(tk + 2 * L::kTile);
     const float* window = reinterpret_cast<const float*>(tk + L::kWindow) + q_off;
     const bool whole = bits == (ROWS == 64 ? ~0ull : 0xffffffffull);
+    const bool line = in_a_row(kt * ROWS, ROWS, p.nk, p.gw);
 #pragma unroll
     for (int u = 0; u < SUBS; ++u) {
       floatx16 s = zero16(), ds = zero16();
@@ -523,16 +563,10 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || (SUMS && DP == 1
         s = mfma(along<T, PITCH>(tk, u * 32 + (lane & 31), 2 * f + hi), qf[f], s);
         ds = mfma(along<T, PITCH>(tv, u * 32 + (lane & 31), 2 * f + hi), df[f], ds);
       }
+      if (sizeof(T) == 4) reads_ahead<2 * KF, 8 * KF, 4>();
+      add_bias<1>(s, p.scale, window, codes, line, window, u, hi);
 #pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const intx4 c = *reinterpret_cast<const intx4*>(codes + u * 32 + 8 * a + 4 * hi);
-        const int cs[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = 4 * a + j;
-          ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale, window[cs[j]]) - m) * fmaf(ds[r], inv, -delta);
-        }
-      }
+      for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(s[r] - m) * fmaf(ds[r], inv, -delta);
       if (!whole) {
         const uint32_t mine = (uint32_t)(bits >> (32 * u)) >> (4 * hi);
 #pragma unroll
@@ -544,19 +578,28 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || (SUMS && DP == 1
         for (int r = 0; r < 16; ++r) diag[(lane & 31) * kDiagRow + kDiagZeros + result_row(r, hi)] = ds[r];
         wave_order();
         float sum[2] = {0.f, 0.f};
-        int col = wave_col;
+        const float* at = diag + lane + (kDiagZeros - 31);  // query i of the wave, key i + lane - 31 of the tile
+        if (SUMS == 1 || (wave_line && in_a_row(kt * ROWS + u * 32, 32, p.nk, p.gw))) {
+          // both in one row of the grid: a difference is one offset, which the first query that has it tells
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {                  // query i of the wave, key i + lane - 31 of the tile
-          const float v = diag[i * (kDiagRow + 1) + lane + (kDiagZeros - 31)];
-          sum[0] += v;
-          if (SUMS == 2) {
-            sum[1] += col + diff_col >= p.gw ? v : 0.f;
+          for (int i = 0; i < 32; ++i) sum[0] += at[i * (kDiagRow + 1)];
+          if (SUMS == 2 && wave_col + max(31 - lane, 0) + diff_col >= p.gw) {
+            sum[1] = sum[0];
+            sum[0] = 0.f;
+          }
+        } else {
+          int col = wave_col;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float v = at[i * (kDiagRow + 1)];
+            const bool wraps = col + diff_col >= p.gw;
+            sum[0] += wraps ? 0.f : v;
+            sum[1] += wraps ? v : 0.f;
             col = col + 1 == p.gw ? 0 : col + 1;
           }
         }
         wave_order();
         if (SUMS == 2) {
-          sum[0] -= sum[1];
           diff_col += step_col;
           if (diff_col >= p.gw) diff_col -= p.gw;
         }
@@ -572,6 +615,7 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || (SUMS && DP == 1
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t) dq[t] = mfma(across<T, PITCH>(tk, u * 32, f, t * 32, lane), sf, dq[t]);
       }
+      if (sizeof(T) == 4) reads_ahead<4 * PF * (DP / 32), 4 * PF * (DP / 32), 8>();
     }
     __syncthreads();
   }
@@ -648,6 +692,8 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || DP == 128 ? 1 : 
     const int* codes = reinterpret_cast<const int*>(tq + 2 * L::kTile);
     const float* rows = reinterpret_cast<const float*>(tq + 2 * L::kTile + L::kRowData);
     const float* window = reinterpret_cast<const float*>(tq + L::kWindow) + k_off;
+    // whole tiles of queries in one row of the grid: the last one's entry is the first
+    const bool line = qt * ROWS + ROWS <= p.nq && in_a_row(p.q_start + qt * ROWS, ROWS, p.nk, p.gw);
 #pragma unroll
     for (int u = 0; u < SUBS; ++u) {
       floatx16 s = zero16(), ds = zero16();
@@ -656,18 +702,17 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 || DP == 128 ? 1 : 
         s = mfma(along<T, PITCH>(tq, u * 32 + (lane & 31), 2 * f + hi), kf[f], s);
         ds = mfma(along<T, PITCH>(td, u * 32 + (lane & 31), 2 * f + hi), vf[f], ds);
       }
+      add_bias<-1>(s, p.scale, window, codes, line, window + ROWS - 1, u, hi);
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
-        const intx4 c = *reinterpret_cast<const intx4*>(codes + u * 32 + 8 * a + 4 * hi);
         const floatx4 e = *reinterpret_cast<const floatx4*>(rows + u * 32 + 8 * a + 4 * hi);
         const floatx4 w = *reinterpret_cast<const floatx4*>(rows + 64 + u * 32 + 8 * a + 4 * hi);
         const floatx4 g = *reinterpret_cast<const floatx4*>(rows + 128 + u * 32 + 8 * a + 4 * hi);
-        const int cs[4] = {c.x, c.y, c.z, c.w};
         const float es[4] = {e.x, e.y, e.z, e.w}, ws[4] = {w.x, w.y, w.z, w.w}, gs[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = 4 * a + j;
-          const float pr = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale, window[cs[j]]) - es[j]);
+          const float pr = __builtin_amdgcn_exp2f(s[r] - es[j]);
           s[r] = pr * ws[j];
           ds[r] = pr * fmaf(ds[r], ws[j], -gs[j]);
         }

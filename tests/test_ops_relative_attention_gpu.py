@@ -7,7 +7,9 @@ exp2, the sum of up to n terms, its inverse).  16-bit types round p by half, and
 its product with v.  out: (rel + half + (n + 2) u) sum p |v| + tiny sum |v|, and half |out|.
 dp: (d + 2) u |do|.|v|;  do.o: the same of |o| and the error of the unrounded o;  ds = p (dp - do.o): rel |ds| and p times
 those two;  dq, dk, dv: sums of |error| |other| and of (n + 2) u |terms|, ds and p rounded by half and tiny first;
-d_table: the sum of ds' errors over its pairs and (n + 64) u sum |ds|."""
+d_table: the sum of ds' errors over its pairs and (n + 64) u sum |ds|.
+Underflow: fp32 instructions give 0 below 2^-126 = flush.  A row's sum has a term of at least 1, so p = exp2(..) / sum is
+off by flush at most; ds = p (dp - do.o) by flush (|dp| + |do.o|) for p and flush for the product itself."""
 import math
 
 import pytest
@@ -17,6 +19,7 @@ from tests import ops_reference as R
 
 pytestmark = pytest.mark.gpu
 
+FLUSH = 2.0 ** -126
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 
 
@@ -58,17 +61,18 @@ def bounds(tensors, buckets, mask, start, do, scale, dtype):
         es = es.masked_fill(~mask[:, None, None], 0)
     rel = 2 * es.amax(-1, keepdim=True) + (n + 24) * R.U
     pv = p @ v.abs()
-    o32 = (rel + (n + 2) * R.U + own) * pv + tiny * v.abs().sum(2, keepdim=True)
+    o32 = (rel + (n + 2) * R.U + own) * pv + (tiny + FLUSH) * v.abs().sum(2, keepdim=True)
     e_out = o32 + half * out.abs() + R.TINY[dtype]
     e_dp = (d + 2) * R.U * (do.abs() @ v.abs().transpose(-1, -2))
     e_delta = ((d + 2) * R.U * do.abs() * out.abs() + do.abs() * o32).sum(-1, keepdim=True)
     ds = mid["ds"]
-    e_ds = (rel + 8 * R.U) * ds.abs() + p * (e_dp + e_delta) + 8 * R.U * p * (mid["dp"].abs() + mid["delta"].abs())
+    e_ds = (rel + 8 * R.U) * ds.abs() + p * (e_dp + e_delta) + 8 * R.U * p * (mid["dp"].abs() + mid["delta"].abs()) + \
+        FLUSH * (mid["dp"].abs() + mid["delta"].abs() + 1)
     e_in = e_ds + own * ds.abs() + tiny
     acc = lambda m: (m + 2) * R.U  # noqa: E731
     e_dq = scale * (e_in @ k.abs() + acc(n) * (ds.abs() @ k.abs()))
     e_dk = scale * (e_in.transpose(-1, -2) @ q.abs() + acc(nq) * (ds.abs().transpose(-1, -2) @ q.abs()))
-    ep = (rel + own + acc(nq)) * p + tiny
+    ep = (rel + own + acc(nq)) * p + tiny + FLUSH
     e_dv = ep.transpose(-1, -2) @ do.abs()
     grow = torch.zeros((table.shape[0] + 1, table.shape[1]), dtype=table.dtype, device=table.device)
     grow.index_add_(0, mid["flat"], (e_ds + (n + 64) * R.U * ds.abs()).sum(0).flatten(1).T)
@@ -120,6 +124,26 @@ def test_many_queries_and_few(gpu_device, dtype):
     check(*make(gpu_device, 16, 8, (11, 17), 32, dtype, seed=1))
     check(*make(gpu_device, 1, 1, (1, 9000), 64, dtype, 1, 4500, seed=2))
     check(*make(gpu_device, 1, 1, (60, 80), 64, dtype, 2, 4700, masked=True, seed=3))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("grid,queries,start", [((5, 64), None, 0), ((3, 96), 200, 33), ((6, 32), 64, 64), ((2, 128), 97, 128)])
+def test_tiles_in_one_row_of_the_grid(gpu_device, grid, queries, start, dtype):
+    """Grids as wide as tiles of keys and queries, wholly, partly and with the queries between two rows."""
+    for masked in (False, True):
+        check(*make(gpu_device, 2, 2, grid, 64, dtype, queries, start, masked, per_axis=40, seed=20))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_a_maximum_that_grows(gpu_device, dtype):
+    """Logits that rise, jump and fall along the keys: by less than 8 powers of two a tile, by many, and back."""
+    t, buckets, mask, start, do = make(gpu_device, 1, 2, (1, 640), 32, dtype, seed=21)
+    n = torch.arange(640, device=gpu_device, dtype=torch.float32)
+    for rise in (n / 40, -n / 40, 12 * (n // 64), 6 * torch.sin(n / 20)):
+        q, k = t[0].clone(), t[1].clone()
+        q[..., 0] = 1
+        k[..., 0] = rise.to(dtype)
+        check([q, k, t[2], t[3]], buckets, mask, start, do, scale=1.0)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
