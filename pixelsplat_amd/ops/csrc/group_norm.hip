@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kThreads) group_norm_apply_kernel(
   const T* p = x + n * rx.sample + q.c0 + q.vec;
   T* o = y + (int64_t)n * sh.s * sh.c + q.c0 + q.vec;
   with_act(sh.act, [&](auto tag) {
-#pragma unroll 4
+#pragma unroll 8
     for (int r = r0 + q.row0; r < r1; r += q.tr) {
       const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(p + r * rx.row);
       Pack<T, V> out;
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kThreads) group_norm_grad_sums_kernel(
     const T* p = x + n * rx.sample + q.c0 + q.vec;
     const T* d = dy + n * rdy.sample + q.c0 + q.vec;
     with_act(sh.act, [&](auto tag) {
-#pragma unroll 2
+#pragma unroll 4
       for (int r = r0 + q.row0; r < r1; r += q.tr) {
         const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(p + r * rx.row);
         const Pack<T, V> u = *reinterpret_cast<const Pack<T, V>*>(d + r * rdy.row);
@@ -388,41 +388,40 @@ __global__ void __launch_bounds__(kThreads) group_norm_grad_sums_kernel(
   }
 }
 
-// Blocks 0 .. n * groups / 4: a wave per (sample, group), group_sums = (mean(gamma dz), mean(gamma dz xh)).
-// The blocks behind them: 16 columns of d_beta | d_gamma each, 16 threads a column.
+// Blocks 0 .. n * groups - 1: a (sample, group), group_sums = (mean(gamma dz), mean(gamma dz xh)).
+// The blocks behind them: 8 columns of d_beta | d_gamma each, 32 threads a column.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) group_norm_fold_kernel(
     Shape sh, int chunks, int group_blocks, const float* __restrict__ partial, const void* __restrict__ gamma,
     float2* __restrict__ group_sums, void* __restrict__ d_gamma, void* __restrict__ d_beta) {
-  __shared__ double lds[16][17];
+  __shared__ double lds[32][9];
   if ((int)blockIdx.x < group_blocks) {
-    const int i = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (i >= sh.n * sh.groups) return;
-    const int n = i / sh.groups, c0 = (i % sh.groups) * sh.cg;
+    __shared__ double2 waves[kThreads / 64];
+    const int n = blockIdx.x / sh.groups, c0 = (blockIdx.x % sh.groups) * sh.cg;
     const float* p = partial + (int64_t)n * chunks * 2 * sh.c;
     double2 t = make_double2(0, 0);
     const int items = chunks * sh.cg;
 #pragma unroll 4
-    for (int j = lane; j < items; j += 64) {
+    for (int j = threadIdx.x; j < items; j += kThreads) {
       const int chunk = j / sh.cg, c = c0 + j % sh.cg;
       const double ga = gamma ? load_param<T>(gamma, sh.param_f32, c) : 1.f;
       t.x += ga * p[(int64_t)(2 * chunk) * sh.c + c];
       t.y += ga * p[(int64_t)(2 * chunk + 1) * sh.c + c];
     }
-    t = wave_sum(t);
+    t = block_sum(t, waves);
     const double inv = 1.0 / ((double)sh.s * sh.cg);
-    if (lane == 0) group_sums[i] = make_float2((float)(t.x * inv), (float)(t.y * inv));
+    if (threadIdx.x == 0) group_sums[blockIdx.x] = make_float2((float)(t.x * inv), (float)(t.y * inv));
     return;
   }
-  const int col = (blockIdx.x - group_blocks) * 16 + (threadIdx.x & 15), l = threadIdx.x >> 4;
+  const int col = (blockIdx.x - group_blocks) * 8 + (threadIdx.x & 7), l = threadIdx.x >> 3;
   double t = 0;
   if (col < 2 * sh.c)
 #pragma unroll 8
-    for (int64_t p = l; p < (int64_t)sh.n * chunks; p += 16) t += partial[p * 2 * sh.c + col];
-  lds[l][threadIdx.x & 15] = t;
+    for (int64_t p = l; p < (int64_t)sh.n * chunks; p += 32) t += partial[p * 2 * sh.c + col];
+  lds[l][threadIdx.x & 7] = t;
   __syncthreads();
   if (l == 0 && col < 2 * sh.c) {
-    for (int k = 1; k < 16; ++k) t += lds[k][threadIdx.x];
+    for (int k = 1; k < 32; ++k) t += lds[k][threadIdx.x];
     void* out = col < sh.c ? d_beta : d_gamma;
     if (out) store_param<T>(out, sh.param_f32, col < sh.c ? col : col - sh.c, (float)t);
   }
@@ -452,7 +451,7 @@ __global__ void __launch_bounds__(kThreads) group_norm_grad_apply_kernel(
   const T* d = dy + n * rdy.sample + q.c0 + q.vec;
   T* o = dx + (int64_t)n * sh.s * sh.c + q.c0 + q.vec;
   with_act(sh.act, [&](auto tag) {
-#pragma unroll 2
+#pragma unroll 4
     for (int r = r0 + q.row0; r < r1; r += q.tr) {
       const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(p + r * rx.row);
       const Pack<T, V> u = *reinterpret_cast<const Pack<T, V>*>(d + r * rdy.row);
@@ -507,7 +506,11 @@ Plan plan(const PsGroupNormDesc& d, const void* x, const void* dy, bool backward
   const int vectors = d.channels / p.vec;
   p.column_blocks = (vectors + kThreads - 1) / kThreads;
   const int at_once = kThreads / (vectors < kThreads ? vectors : kThreads);   // rows a block takes at a time
-  int want = (1024 + d.samples * p.column_blocks - 1) / (d.samples * p.column_blocks);
+  // Blocks: four a CU, and up to 16 of 32 steps or more each, so that a CU always has some that read while others end
+  // (14 x 256 x 256 x 256 in bf16: 1040 us at 1024 blocks, 890 at 3584).
+  const int64_t steps = (int64_t)d.samples * p.column_blocks * (d.rows / at_once);
+  const int blocks = steps >= 4096 * 32 ? 4096 : steps >= 1024 * 32 ? (int)(steps / 32) : 1024;
+  int want = (int)((blocks + (int64_t)d.samples * p.column_blocks - 1) / ((int64_t)d.samples * p.column_blocks));
   if (want > 256) want = 256;
   int rows = (d.rows + want - 1) / want;
   rows = round_up(rows < 2 * at_once ? 2 * at_once : rows, at_once);
@@ -546,8 +549,8 @@ void backward_chunks(const PsGroupNormDesc& d, const Plan& p, const void* x, con
   float* partial = reinterpret_cast<float*>(group_sums + (size_t)d.samples * d.groups);
   group_norm_grad_sums_kernel<T, V><<<grid, kThreads, 0, st>>>(sh, p.rows, (const T*)x, rx, (const T*)dy, rdy, gamma,
                                                                beta, mean, rstd, partial);
-  const int group_blocks = (d.samples * d.groups + 3) / 4;
-  group_norm_fold_kernel<T><<<group_blocks + (2 * d.channels + 15) / 16, kThreads, 0, st>>>(
+  const int group_blocks = d.samples * d.groups;
+  group_norm_fold_kernel<T><<<group_blocks + (2 * d.channels + 7) / 8, kThreads, 0, st>>>(
       sh, p.chunks, group_blocks, partial, gamma, group_sums, d_gamma, d_beta);
   group_norm_grad_apply_kernel<T, V><<<grid, kThreads, 0, st>>>(sh, p.rows, (const T*)x, rx, (const T*)dy, rdy, gamma,
                                                                 beta, mean, rstd, group_sums, (T*)dx);
@@ -592,7 +595,7 @@ void backward_typed(const PsGroupNormDesc& d, const void* x, const void* dy, con
       group_norm_held_backward_kernel<T, V, kHeldBackward><<<grid, p.threads, lds, st>>>(
           sh, (const T*)x, rx, (const T*)dy, rdy, gamma, beta, mean, rstd, (T*)dx, partial);
     if (d_gamma || d_beta)
-      group_norm_fold_kernel<T><<<(2 * d.channels + 15) / 16, kThreads, 0, st>>>(sh, 1, 0, partial, gamma, nullptr,
+      group_norm_fold_kernel<T><<<(2 * d.channels + 7) / 8, kThreads, 0, st>>>(sh, 1, 0, partial, gamma, nullptr,
                                                                                  d_gamma, d_beta);
   } else if (p.vec > 1) {
     backward_chunks<T, V>(d, p, x, dy, gamma, beta, mean, rstd, dx, d_gamma, d_beta, workspace, st);
