@@ -757,14 +757,32 @@ __global__ void __launch_bounds__(256) join_diagonals_kernel(Args p, int sums, d
     const float* rows = p.diag_rows + (dx < 0 ? p.diag_pitch : 0) * (sums - 1);
     const int len = p.diag_pitch - 32, end = p.diag_end;        // a split's keys; what the waves' rows hold
     // the waves whose rows hold the difference
-    const int w0 = at < 0 ? (-at + 31) / 32 : 0, w1 = at >= end ? 0 : min(waves, (end - 1 - at) / 32 + 1), n = max(w1 - w0, 0);
+    const int w0 = at < 0 ? (-at + 31) / 32 : 0, w1 = at >= end ? 0 : min(waves, (end - 1 - at) / 32 + 1);
+    const int n = max(w1 - w0, 1), all = w1 > w0 ? p.batch * n : 0;
+    const int64_t pitch_w = (int64_t)p.splits * sums * p.diag_pitch;
+    // (batch, wave) number part, part + 16, ..: a division here, none in the loop
+    int b = part / n, w = part - b * n;
+    const int step_b = 16 / n, step_w = 16 - step_b * n;
+    const float* of_h = rows + (int64_t)h * per * pitch_w;
+    const int64_t pitch_b = (int64_t)p.heads * per * pitch_w;
 #pragma unroll 4
-    for (int i = part; i < p.batch * n; i += 16) {
-      const int b = i / n, w = w0 + i % n, u = at + 32 * w;
-      const int s = min(u / len, p.splits - 1), in = u - s * len;
-      const float* row = rows + (((int64_t)(b * p.heads + h) * per + w) * p.splits + s) * sums * p.diag_pitch;
-      t += row[in];
-      if (s > 0 && in < 32) t += row[in + len - (int64_t)sums * p.diag_pitch];   // the end of the split before
+    for (int i = part; i < all; i += 16) {
+      const float* row = of_h + b * pitch_b + (w0 + w) * pitch_w;
+      const int u = at + 32 * (w0 + w);
+      if (p.splits == 1) {
+        t += row[u];
+      } else {
+        const int s = min(u / len, p.splits - 1), in = u - s * len;
+        row += (int64_t)s * sums * p.diag_pitch;
+        t += row[in];
+        if (s > 0 && in < 32) t += row[in + len - (int64_t)sums * p.diag_pitch];   // the end of the split before
+      }
+      b += step_b;
+      w += step_w;
+      if (w >= n) {
+        w -= n;
+        ++b;
+      }
     }
   }
   lds[part][threadIdx.x & 15] = t;
@@ -805,40 +823,46 @@ __global__ void __launch_bounds__(256) join_gradients_kernel(Gradients a) {
   }
 }
 
-constexpr int kJoinHeads = 8;
+constexpr int kJoinHeads = 8, kJoinList = 8192;
 
-// d_table[bucket][head]: a block a bucket and 8 heads; every block reads the map, 8 entries a thread at a time
+// d_table[bucket][head]: a block a bucket and 8 heads.  It lists the offsets of its bucket, in order -- kJoinList entries
+// of the map at a time, a run of them a wave -- then 32 threads a head take the list's entries.
 template <typename T>
 __global__ void __launch_bounds__(256) join_offsets_kernel(int heads, int offsets, int buckets, const int32_t* __restrict__ map,
                                                            const double* __restrict__ d_offsets, void* __restrict__ d_table,
                                                            int table_f32) {
-  __shared__ double lds[4][kJoinHeads];
-  const int bucket = blockIdx.x, lane = threadIdx.x & 63, h0 = blockIdx.y * kJoinHeads;
-  double t[kJoinHeads];
+  constexpr int kRun = kJoinList / 4;
+  __shared__ int list[4][kRun];
+  __shared__ int found[4];
+  __shared__ double lds[32][kJoinHeads + 1];
+  const int bucket = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int j = threadIdx.x & (kJoinHeads - 1), h = blockIdx.y * kJoinHeads + j, part = threadIdx.x / kJoinHeads;
+  const double* of_h = d_offsets + (int64_t)min(h, heads - 1) * offsets;
+  double t = 0;
+  for (int base = 0; base < offsets; base += kJoinList) {
+    int mine[kRun / 64], n = 0;
+    const int from = base + wave * kRun + lane;
 #pragma unroll
-  for (int j = 0; j < kJoinHeads; ++j) t[j] = 0;
-  for (int base = threadIdx.x; base < offsets; base += 256 * 8) {
-    int mine[8];
+    for (int i = 0; i < kRun / 64; ++i) mine[i] = from + i * 64 < offsets ? map[from + i * 64] : -1;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) mine[i] = base + i * 256 < offsets ? map[base + i * 256] : -1;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (mine[i] == bucket) {
-#pragma unroll
-        for (int j = 0; j < kJoinHeads; ++j)
-          if (h0 + j < heads) t[j] += d_offsets[(int64_t)(h0 + j) * offsets + base + i * 256];
-      }
+    for (int i = 0; i < kRun / 64; ++i) {
+      const uint64_t hits = __ballot(mine[i] == bucket);
+      if (mine[i] == bucket) list[wave][n + __popcll(hits & ((1ull << lane) - 1))] = from + i * 64;
+      n += __popcll(hits);
+    }
+    if (lane == 0) found[wave] = n;
+    __syncthreads();
+    for (int w = 0; w < 4; ++w)
+#pragma unroll 4
+      for (int i = part; i < found[w]; i += 32) t += of_h[list[w][i]];
+    __syncthreads();
   }
-#pragma unroll
-  for (int j = 0; j < kJoinHeads; ++j) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) t[j] += __shfl_xor(t[j], m);
-    if (lane == 0) lds[threadIdx.x >> 6][j] = t[j];
-  }
+  lds[part][j] = t;
   __syncthreads();
-  const int j = threadIdx.x;
-  if (j < kJoinHeads && h0 + j < heads)
-    store_param<T>(d_table, table_f32, (int64_t)bucket * heads + h0 + j, (float)((lds[0][j] + lds[1][j]) + (lds[2][j] + lds[3][j])));
+  if (part == 0 && h < heads) {
+    for (int k = 1; k < 32; ++k) t += lds[k][j];
+    store_param<T>(d_table, table_f32, (int64_t)bucket * heads + h, (float)t);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
