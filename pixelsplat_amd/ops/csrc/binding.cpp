@@ -475,7 +475,8 @@ Tensor relative_attention(const Tensor& q, const Tensor& k, const Tensor& v, con
   need_value(!mask.defined() || (mask.scalar_type() == at::kBool && mask.dim() == 2 && mask.size(0) == b && mask.size(1) == gh * gw),
              "relative_attention: key_mask is [", b, ", ", gh * gw, "] bool, got ", mask.defined() ? shape(mask) : "", " ",
              mask.defined() ? mask.scalar_type() : at::kBool);
-  need_value(h <= 65535 && b * h <= 1 << 24, "relative_attention: at most 65535 heads and 2^24 heads in the batch");
+  need_value(h <= 65535 && b * h < 1 << 24 && b * h * ((std::max(n, gh * gw) + 63) / 64 * 2) < 1 << 26,
+             "relative_attention: at most 65535 heads, and less than 2^24 heads and 2^26 tiles of 32 tokens in the batch");
   check_device("relative_attention", q, {{"k", &k}, {"v", &v}, {"table", &table}, {"buckets", &buckets0}, {"key_mask", &mask}});
   const double scale = scale0 ? *scale0 : 1.0 / std::sqrt((double)dim);
   const Tensor buckets = buckets0.contiguous();

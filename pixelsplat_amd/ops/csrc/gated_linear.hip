@@ -37,7 +37,7 @@ struct Product {
   int halves;             // of the contraction index
   int first;              // blockIdx.z + first: which of a's matrices, where halves is 1
   Operand a, b;
-  int tiles_m, tiles_n, splits, slices_per_split;
+  int tiles_m, tiles_n, slices_per_split;
 };
 
 // which columns of a forward block belong to which projection
@@ -496,7 +496,7 @@ Tiling tiling(int dtype, int m, int columns, int k, int halves, int products, bo
   const int kk = kSliceBytes / (dtype == PS_DTYPE_F32 ? 4 : 2);
   auto count = [](int a, int b) { return (a + b - 1) / b; };
   auto tiles = [&](int size) { return (int64_t)count(m, size) * count(columns, size) * products; };
-    t.bm = dtype != PS_DTYPE_F32 && tiles(256) >= 2 * kCus ? 256 : tiles(128) >= kCus ? 128 : 64;
+  t.bm = dtype != PS_DTYPE_F32 && tiles(256) >= 2 * kCus ? 256 : tiles(128) >= kCus ? 128 : 64;
   t.bn = t.bm;
   t.tiles_m = count(m, t.bm);
   t.tiles_n = count(columns, t.bn);
@@ -516,7 +516,6 @@ template <typename T, bool A_ACROSS, bool B_ACROSS, bool PAIRED, typename EP>
 int launch_product(Product g, const Tiling& t, const EP& ep, hipStream_t st, int products = 1) {
   g.tiles_m = t.tiles_m;
   g.tiles_n = t.tiles_n;
-  g.splits = t.splits;
   g.slices_per_split = t.slices_per_split;
   const dim3 grid((unsigned)(t.tiles_m * t.tiles_n), (unsigned)t.splits, (unsigned)products);
   // two buffers of slices; then at most two staged tiles of half the columns, or one of all
@@ -559,6 +558,7 @@ BackwardPlan backward_plan(const PsGatedLinearDesc& d) {
   p.dw = tiling(d.dtype, d.hidden, d.dim, d.rows, 1, 2, true);
   p.slope_rows = 8;
   while (p.slope_rows < 64 && (int64_t)d.rows * p.ld > (int64_t)p.slope_rows * 256 * 8 * kCus) p.slope_rows *= 2;
+  while (d.rows / p.slope_rows >= 32768) p.slope_rows *= 2;   // blocks along a grid's second axis
   p.sum_parts = d.dtype == PS_DTYPE_F32 ? (d.rows + p.slope_rows - 1) / p.slope_rows : p.again.tiles_m * 2;
   size_t at = 0;
   p.da = at; at += align256(e * d.rows * p.ld);

@@ -1057,11 +1057,12 @@ int check(const PsRelativeAttentionDesc* d) {
   if (d->dtype < PS_DTYPE_F32 || d->dtype > PS_DTYPE_F16) return PS_ERR_UNSUPPORTED;
   const int64_t nk = (int64_t)d->grid_h * d->grid_w;
   if (nk > 1 << 20 || (d->grid_h > 1 && d->grid_w > 512) || d->dim > 128 || d->heads > 65535 ||
-      (int64_t)d->batch * d->heads > 1 << 24 || d->buckets > 1 << 24)
+      (int64_t)d->batch * d->heads >= 1 << 24 || d->buckets > 1 << 24)
     return PS_ERR_UNSUPPORTED;
   if (d->query_start + (int64_t)d->queries > nk) return PS_ERR_BAD_ARG;
-  if ((int64_t)d->batch * d->heads * ((d->queries + 63) / 64 * 2) >= 1 << 30 ||
-      (int64_t)d->batch * d->heads * ((nk + 31) / 32) >= 1 << 30)
+  // threads of a launch: 64 for 32 tokens, 256 at least for a head, 2^32 at most
+  if ((int64_t)d->batch * d->heads * ((d->queries + 63) / 64 * 2) >= 1 << 26 ||
+      (int64_t)d->batch * d->heads * ((nk + 31) / 32) >= 1 << 26)
     return PS_ERR_UNSUPPORTED;
   const int chunk = d->dtype == PS_DTYPE_F32 ? 4 : 8;
   if (d->dim % chunk) return PS_ERR_BAD_ARG;

@@ -83,7 +83,8 @@ int ps_gated_linear_backward(const PsGatedLinearDesc* desc, const void* x, const
  * For the backward the forward leaves bias [heads][offsets] fp32 (always written), stats [2][batch][heads][queries
  * rounded up to 64] fp32 and out_f32 (the unrounded out; fp32 tensors hand `out` itself to the backward and NULL to the
  * forward); stats and out_f32 are NULL where no backward follows.  Backward: each output may be NULL.
- * dim <= 128, keys <= 2^20, grid_w <= 512 unless grid_h is 1, token strides < 2^24 (else PS_ERR_UNSUPPORTED). */
+ * dim <= 128, keys <= 2^20, grid_w <= 512 unless grid_h is 1, token strides < 2^24, batch * heads < 2^24 and
+ * batch * heads * tokens / 32 < 2^26, tokens rounded up to whole tiles (else PS_ERR_UNSUPPORTED). */
 typedef struct PsRelativeAttentionDesc {
   int32_t batch, heads, queries, query_start, grid_h, grid_w, dim;
   int32_t dtype, buckets, table_f32;

@@ -236,6 +236,10 @@ def test_relative_attention_c_abi_refusals(lib):
         bad = _lib.PsRelativeAttentionDesc(**{**good, field: value})
         assert forward(bad) == status and backward(bad) == status, field
         assert lib.ps_relative_attention_workspace_bytes(C.byref(bad), 1) == 0
+    for more in (dict(batch=1 << 13, heads=1 << 11), dict(batch=1 << 10, heads=64, queries=1, grid_h=1, grid_w=1 << 15)):
+        bad = _lib.PsRelativeAttentionDesc(**{**good, **more})
+        assert forward(bad) == backward(bad) == -4, more
+        assert lib.ps_relative_attention_workspace_bytes(C.byref(bad), 0) == 0
     for strides, status in [(three(96, 8, 20), -1), (three(-96, 8, 24), -1), (three(96, 8, 1 << 24), -4)]:
         assert forward(_lib.PsRelativeAttentionDesc(**{**good, "k_strides": strides})) == status
         assert backward(_lib.PsRelativeAttentionDesc(**{**good, "do_strides": strides})) == status

@@ -93,6 +93,11 @@ def test_large_tiles(gpu_device, dtype):
     check(*make(gpu_device, 300, 5000, 6200, dtype, seed=3, bias=False), "gelu")
 
 
+def test_many_rows(gpu_device):
+    """More parts of 64 rows than a grid's second axis holds."""
+    check(*make(gpu_device, (1 << 22) + 3, 8, 8, torch.float32, seed=12), "silu")
+
+
 @pytest.mark.parametrize("which", ["gate", "up"])
 def test_one_bias(gpu_device, which):
     t, dh = make(gpu_device, 70, 64, 48, torch.bfloat16, seed=4)
