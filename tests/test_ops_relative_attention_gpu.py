@@ -127,6 +127,13 @@ def test_many_queries_and_few(gpu_device, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_a_last_round_of_few_blocks(gpu_device, dtype):
+    """A few blocks more than there are CUs, which split what they stream: queries, keys or both in uneven parts."""
+    check(*make(gpu_device, 3, 9, (33, 40), 32 if dtype == torch.float32 else 128, dtype, masked=True, seed=22))
+    check(*make(gpu_device, 3, 9, (33, 40), 128, dtype, 1300, 11, seed=23))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("grid,queries,start", [((5, 64), None, 0), ((3, 96), 200, 33), ((6, 32), 64, 64), ((2, 128), 97, 128)])
 def test_tiles_in_one_row_of_the_grid(gpu_device, grid, queries, start, dtype):
     """Grids as wide as tiles of keys and queries, wholly, partly and with the queries between two rows."""
