@@ -59,8 +59,8 @@ def relative_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, buckets: 
     zero.  scale: dim ** -0.5 by default.  Returns [batch, heads, queries, dim], token-major in memory.
 
     dim <= 128, at most 2^20 keys, gw <= 512 on grids of more than one row.  Differentiable once in q, k, v and table;
-    the gradient of the table is summed over the batch.  16-bit types accumulate in fp32 and round probabilities for
-    their product with v.  Results repeat bit for bit."""
+    the gradient of the table is summed over the batch.  16-bit types accumulate in fp32; the
+    backward rounds probabilities and the logits' gradients to them for its products.  Results repeat bit for bit."""
     return _lib.binding().relative_attention(q, k, v, table, buckets, key_mask, scale, query_start)
 
 

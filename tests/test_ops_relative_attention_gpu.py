@@ -3,8 +3,9 @@
 Bounds, from the arithmetic; u = 2^-24, half = half a step of the result's type, n keys, d the head's width.  A logit is
 off by es = (d + 8) u scale |q|.|k| + 8 u |bias| (a product of d terms, the factor log2(e) on scale and bias, their
 sum); a probability, relative to itself, by rel = 2 max(es) + (n + 24) u (its own logit and the others' in the sum,
-exp2, the sum of up to n terms, its inverse).  16-bit types round p by half, and where it is subnormal by `tiny`, before
-its product with v.  out: (rel + half + (n + 2) u) sum p |v| + tiny sum |v|, and half |out|.
+exp2, the sum of up to n terms, its inverse).  16-bit types split p into its rounding and the rounded rest, off by
+half^2, and by `tiny` where that is subnormal, before its product with v.  out: (rel + half^2 + (n + 2) u) sum p |v| +
+tiny sum |v|, and half |out|.
 dp: (d + 2) u |do|.|v|;  do.o: the same of |o| and the error of the unrounded o;  ds = p (dp - do.o): rel |ds| and p times
 those two;  dq, dk, dv: sums of |error| |other| and of (n + 2) u |terms|, ds and p rounded by half and tiny first;
 d_table: the sum of ds' errors over its pairs and (n + 64) u sum |ds|.
@@ -61,7 +62,7 @@ def bounds(tensors, buckets, mask, start, do, scale, dtype):
         es = es.masked_fill(~mask[:, None, None], 0)
     rel = 2 * es.amax(-1, keepdim=True) + (n + 24) * R.U
     pv = p @ v.abs()
-    o32 = (rel + (n + 2) * R.U + own) * pv + (tiny + FLUSH) * v.abs().sum(2, keepdim=True)
+    o32 = (rel + (n + 2) * R.U + own ** 2) * pv + (tiny + FLUSH) * v.abs().sum(2, keepdim=True)
     e_out = o32 + half * out.abs() + R.TINY[dtype]
     e_dp = (d + 2) * R.U * (do.abs() @ v.abs().transpose(-1, -2))
     e_delta = ((d + 2) * R.U * do.abs() * out.abs() + do.abs() * o32).sum(-1, keepdim=True)
