@@ -220,20 +220,29 @@ struct Columns {
   }
 };
 
+// The rows of a chunk.  A sample may have up to 2^31 - 1: the end of the last chunk does not fit 32 bits, so rows are
+// counted from the chunk's first.
+struct Chunk {
+  int64_t first;
+  int count;
+  __device__ Chunk(int s, int rows, int chunk) : first((int64_t)chunk * rows), count((int)min((int64_t)rows, s - first)) {}
+};
+
 // sums: [n][chunks * column blocks][groups] of (sum x, sum x^2)
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) group_norm_sums_kernel(Shape sh, int rows, const T* __restrict__ x, Rows rx,
                                                                   double2* __restrict__ sums) {
   __shared__ double2 lds[kThreads * V];
   const Columns q(sh.c, V, blockIdx.z);
-  const int n = blockIdx.y, r0 = blockIdx.x * rows, r1 = min(r0 + rows, sh.s);
+  const Chunk k(sh.s, rows, blockIdx.x);
+  const int n = blockIdx.y;
   double2 acc[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) acc[e] = make_double2(0, 0);
   if (q.on) {
-    const T* p = x + n * rx.sample + q.c0 + q.vec;
+    const T* p = x + n * rx.sample + k.first * rx.row + q.c0 + q.vec;
 #pragma unroll 4
-    for (int r = r0 + q.row0; r < r1; r += q.tr) {
+    for (int r = q.row0; r < k.count; r += q.tr) {
       const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(p + r * rx.row);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
@@ -303,7 +312,7 @@ __global__ void __launch_bounds__(kThreads) group_norm_apply_kernel(
   const Columns q(sh.c, V, blockIdx.z);
   // opposite order of the sums kernel: what it read last comes first
   const int n = gridDim.y - 1 - blockIdx.y, chunk = gridDim.x - 1 - blockIdx.x;
-  const int r0 = chunk * rows, r1 = min(r0 + rows, sh.s);
+  const Chunk k(sh.s, rows, chunk);
   fold_moments(sh, parts, sums + (int64_t)n * parts * sh.groups, scratch, stats);
   if (chunk == 0 && blockIdx.z == 0)
     for (int g = threadIdx.x; g < sh.groups; g += kThreads) {
@@ -320,11 +329,11 @@ __global__ void __launch_bounds__(kThreads) group_norm_apply_kernel(
     scale[e] = st.y * (gamma ? load_param<T>(gamma, sh.param_f32, c) : 1.f);
     be[e] = beta ? load_param<T>(beta, sh.param_f32, c) : 0.f;
   }
-  const T* p = x + n * rx.sample + q.c0 + q.vec;
-  T* o = y + (int64_t)n * sh.s * sh.c + q.c0 + q.vec;
+  const T* p = x + n * rx.sample + k.first * rx.row + q.c0 + q.vec;
+  T* o = y + ((int64_t)n * sh.s + k.first) * sh.c + q.c0 + q.vec;
   with_act(sh.act, [&](auto tag) {
 #pragma unroll 8
-    for (int r = r0 + q.row0; r < r1; r += q.tr) {
+    for (int r = q.row0; r < k.count; r += q.tr) {
       const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(p + r * rx.row);
       Pack<T, V> out;
 #pragma unroll
@@ -343,7 +352,8 @@ __global__ void __launch_bounds__(kThreads) group_norm_grad_sums_kernel(
     const float* __restrict__ rstd_in, float* __restrict__ partial) {
   __shared__ float lds[2][kThreads * V];
   const Columns q(sh.c, V, blockIdx.z);
-  const int n = blockIdx.y, r0 = blockIdx.x * rows, r1 = min(r0 + rows, sh.s);
+  const Chunk k(sh.s, rows, blockIdx.x);
+  const int n = blockIdx.y;
   if (q.on) {
     float mean[V], rstd[V], ga[V], be[V], sb[V], sg[V];
 #pragma unroll
@@ -355,11 +365,11 @@ __global__ void __launch_bounds__(kThreads) group_norm_grad_sums_kernel(
       be[e] = beta ? load_param<T>(beta, sh.param_f32, c) : 0.f;
       sb[e] = sg[e] = 0.f;
     }
-    const T* p = x + n * rx.sample + q.c0 + q.vec;
-    const T* d = dy + n * rdy.sample + q.c0 + q.vec;
+    const T* p = x + n * rx.sample + k.first * rx.row + q.c0 + q.vec;
+    const T* d = dy + n * rdy.sample + k.first * rdy.row + q.c0 + q.vec;
     with_act(sh.act, [&](auto tag) {
 #pragma unroll 4
-      for (int r = r0 + q.row0; r < r1; r += q.tr) {
+      for (int r = q.row0; r < k.count; r += q.tr) {
         const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(p + r * rx.row);
         const Pack<T, V> u = *reinterpret_cast<const Pack<T, V>*>(d + r * rdy.row);
 #pragma unroll
@@ -382,10 +392,10 @@ __global__ void __launch_bounds__(kThreads) group_norm_grad_sums_kernel(
   float* out = partial + ((int64_t)n * gridDim.x + blockIdx.x) * 2 * sh.c;
   for (int c = threadIdx.x; c < q.nc; c += kThreads) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int j = 0; j < 2; ++j) {
       float t = 0.f;
-      for (int r = 0; r < q.tr; ++r) t += lds[k][r * q.nc + c];
-      out[k * sh.c + q.c0 + c] = t;
+      for (int r = 0; r < q.tr; ++r) t += lds[j][r * q.nc + c];
+      out[j * sh.c + q.c0 + c] = t;
     }
   }
 }
@@ -436,7 +446,7 @@ __global__ void __launch_bounds__(kThreads) group_norm_grad_apply_kernel(
     const float* __restrict__ rstd_in, const float2* __restrict__ group_sums, T* __restrict__ dx) {
   const Columns q(sh.c, V, blockIdx.z);
   const int n = gridDim.y - 1 - blockIdx.y, chunk = gridDim.x - 1 - blockIdx.x;
-  const int r0 = chunk * rows, r1 = min(r0 + rows, sh.s);
+  const Chunk k(sh.s, rows, chunk);
   if (!q.on) return;
   float mean[V], rstd[V], ga[V], be[V], m1[V], m2[V];
 #pragma unroll
@@ -449,12 +459,12 @@ __global__ void __launch_bounds__(kThreads) group_norm_grad_apply_kernel(
     m1[e] = group_sums[g].x;
     m2[e] = group_sums[g].y;
   }
-  const T* p = x + n * rx.sample + q.c0 + q.vec;
-  const T* d = dy + n * rdy.sample + q.c0 + q.vec;
-  T* o = dx + (int64_t)n * sh.s * sh.c + q.c0 + q.vec;
+  const T* p = x + n * rx.sample + k.first * rx.row + q.c0 + q.vec;
+  const T* d = dy + n * rdy.sample + k.first * rdy.row + q.c0 + q.vec;
+  T* o = dx + ((int64_t)n * sh.s + k.first) * sh.c + q.c0 + q.vec;
   with_act(sh.act, [&](auto tag) {
 #pragma unroll 4
-    for (int r = r0 + q.row0; r < r1; r += q.tr) {
+    for (int r = q.row0; r < k.count; r += q.tr) {
       const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(p + r * rx.row);
       const Pack<T, V> u = *reinterpret_cast<const Pack<T, V>*>(d + r * rdy.row);
       Pack<T, V> out;
@@ -477,7 +487,7 @@ struct Plan {
   int chunks, rows, column_blocks;
 };
 
-int round_up(int a, int b) { return (a + b - 1) / b * b; }
+int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
 Plan plan(const PsGroupNormDesc& d, const void* x, const void* dy, bool backward) {
   Plan p = {};
@@ -514,10 +524,10 @@ Plan plan(const PsGroupNormDesc& d, const void* x, const void* dy, bool backward
   const int blocks = steps >= 4096 * 32 ? 4096 : steps >= 1024 * 32 ? (int)(steps / 32) : 1024;
   int want = (int)((blocks + (int64_t)d.samples * p.column_blocks - 1) / ((int64_t)d.samples * p.column_blocks));
   if (want > 256) want = 256;
-  int rows = (d.rows + want - 1) / want;
+  int64_t rows = ((int64_t)d.rows + want - 1) / want;
   rows = round_up(rows < 2 * at_once ? 2 * at_once : rows, at_once);
-  p.rows = rows;
-  p.chunks = (d.rows + rows - 1) / rows;
+  p.rows = (int)(rows < d.rows ? rows : d.rows);
+  p.chunks = (int)((d.rows + rows - 1) / rows);
   return p;
 }
 

@@ -269,3 +269,15 @@ def test_encoder_modules_take_the_operators_when_asked(lib):
         Attention(8, 2, 4, selfatt=False, kv_dim=8, relative_buckets=8)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         GatedFeedForward(8, 16)(torch.zeros(2, 8))
+
+
+def test_group_norm_workspace_of_the_longest_samples(lib):
+    """Up to 2^31 - 1 rows: the chunks' number, and with it the workspace, stays what it is at 2^30."""
+    from pixelsplat_amd.ops import _lib
+    for rows in ((1 << 31) - 1, (1 << 31) - 255, 2147418113):
+        for dtype in (0, 1):
+            size = [lib.ps_group_norm_workspace_bytes(C.byref(_lib.PsGroupNormDesc(
+                samples=1, rows=r, channels=1, groups=1, dtype=dtype, activation=0, param_f32=1, eps=1e-5,
+                x_sample_stride=0, x_row_stride=1, dy_sample_stride=0, dy_row_stride=1)), b) for r in (rows, 1 << 30)
+                for b in (0, 1)]
+            assert 0 < size[0] <= 2 * size[2] and 0 < size[1] <= 2 * size[3], (rows, size)
