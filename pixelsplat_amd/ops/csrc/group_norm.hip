@@ -12,8 +12,8 @@
 //    y 212 (4.4), gradient's sums 255 (3.7), dx 278 (5.1, some of it from that cache).  Passing a few samples at a time
 //    through both passes, all of them from the cache, took 1716 us: launches that small do not fill the memory.
 // Sums over x and x^2 are held in 64 bits: E[x^2] - mean^2 then needs no pivot, whatever the mean is, and the double
-// adds hide under the loads.  The backward's sums are fp32 within a chunk (at most a few hundred terms a thread) and
-// 64 bits across chunks.  Every sum has a fixed order: results repeat bit for bit.
+// adds hide under the loads.  The backward's sums are fp32 within a thread (at most 256 rows) and 64 bits across threads and
+// chunks, whose sums are rounded to fp32 once each.  Every sum has a fixed order: results repeat bit for bit.
 #include "elem.h"
 #include "pixelsplat_ops.h"
 
@@ -393,9 +393,9 @@ __global__ void __launch_bounds__(kThreads) group_norm_grad_sums_kernel(
   for (int c = threadIdx.x; c < q.nc; c += kThreads) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      float t = 0.f;
+      double t = 0;
       for (int r = 0; r < q.tr; ++r) t += lds[j][r * q.nc + c];
-      out[j * sh.c + q.c0 + c] = t;
+      out[j * sh.c + q.c0 + c] = (float)t;
     }
   }
 }
@@ -524,6 +524,9 @@ Plan plan(const PsGroupNormDesc& d, const void* x, const void* dy, bool backward
   const int blocks = steps >= 4096 * 32 ? 4096 : steps >= 1024 * 32 ? (int)(steps / 32) : 1024;
   int want = (int)((blocks + (int64_t)d.samples * p.column_blocks - 1) / ((int64_t)d.samples * p.column_blocks));
   if (want > 256) want = 256;
+  // the gradient's sums are fp32 within a thread: no more than 256 rows of it, however long the sample
+  const int64_t least = ((int64_t)d.rows + (int64_t)at_once * 256 - 1) / ((int64_t)at_once * 256);
+  if (backward && want < least) want = (int)least;
   int64_t rows = ((int64_t)d.rows + want - 1) / want;
   rows = round_up(rows < 2 * at_once ? 2 * at_once : rows, at_once);
   p.rows = (int)(rows < d.rows ? rows : d.rows);

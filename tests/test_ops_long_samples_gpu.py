@@ -40,6 +40,7 @@ def test_the_longest_sample(gpu_device):
     dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
     top = (3 - mean) * rstd
     assert abs(db.item() - tail) <= 320 * R.U * tail
+    assert abs(dw.item() - tail * top) <= 330 * R.U * tail * top
     m1, m2 = tail / n, tail * top / n
     half, tiny = R.HALF_STEP[torch.float16], R.TINY[torch.float16]
     for a in range(0, n, PART):
@@ -50,3 +51,23 @@ def test_the_longest_sample(gpu_device):
         ref = rstd * (dy[0, part, 0].float() - m1 - xh * m2)
         over = (dx[0, part, 0].float() - ref).abs() - (half * ref.abs() + 400 * R.U * rstd * 8 + tiny)
         assert (over <= 0).all(), a
+
+
+@pytest.mark.parametrize("c,groups,dtype", [(1, 1, torch.float32), (8, 2, torch.bfloat16)])
+def test_sums_of_long_samples(gpu_device, c, groups, dtype):
+    """The gradient's sums over 2^28 rows, of equal terms, whose roundings do not cancel: a thread adds 256 of them in fp32,
+    and its sum, a block's and the result are rounded once each (260 roundings of 2^-24 of the sum at most)."""
+    from pixelsplat_amd.ops import group_norm
+
+    n = (1 << 28) // c
+    x = torch.ones((1, n, c), dtype=dtype, device=gpu_device)
+    x[:, ::2] = -1
+    x.requires_grad_()
+    w, b = torch.ones(c, device=gpu_device, requires_grad=True), torch.zeros(c, device=gpu_device, requires_grad=True)
+    dy = torch.full((1, 1, 1), 0.7, dtype=dtype, device=gpu_device)
+    dw, db = torch.autograd.grad(group_norm(x, groups, w, b), (w, b), dy.expand(1, n, c))
+    want = n * dy.item()
+    assert ((db.double() - want).abs() <= 260 * R.U * want).all(), (db.double() - want).abs().max().item() / want / R.U
+    dw1 = torch.autograd.grad(group_norm(x, groups, w, b), w, x.detach())[0]      # xh = x rstd: terms of rstd
+    want = n / math.sqrt(1 + 1e-5)
+    assert ((dw1.double() - want).abs() <= 264 * R.U * want).all(), (dw1.double() - want).abs().max().item() / want / R.U
