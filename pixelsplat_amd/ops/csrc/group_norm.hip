@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(1024) group_norm_held_forward_kernel(
     Shape sh, const T* __restrict__ x, Rows rx, const void* __restrict__ gamma, const void* __restrict__ beta,
     T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
   __shared__ double2 lds[16];
-  const int n = blockIdx.x / sh.groups, g = blockIdx.x % sh.groups;
+  const int g = blockIdx.x, n = blockIdx.y, at = n * sh.groups + g;
   const int per_row = sh.cg / V, count = sh.s * per_row;
   const T* xg = x + n * rx.sample + (int64_t)g * sh.cg;
   T* yg = y + ((int64_t)n * sh.s * sh.groups + g) * sh.cg;
@@ -97,8 +97,8 @@ __global__ void __launch_bounds__(1024) group_norm_held_forward_kernel(
   float mean, rstd;
   moments(block_sum(sum, lds), (double)sh.s * sh.cg, sh.eps, mean, rstd);
   if (threadIdx.x == 0) {
-    mean_out[blockIdx.x] = mean;
-    rstd_out[blockIdx.x] = rstd;
+    mean_out[at] = mean;
+    rstd_out[at] = rstd;
   }
   with_act(sh.act, [&](auto tag) {
 #pragma unroll
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(1024) group_norm_held_backward_kernel(
     T* __restrict__ dx, float* __restrict__ partial) {
   extern __shared__ float chan[];                     // [rows in flight][2][cg]
   __shared__ double2 lds[16];
-  const int n = blockIdx.x / sh.groups, g = blockIdx.x % sh.groups;
+  const int g = blockIdx.x, n = blockIdx.y, at = n * sh.groups + g;
   const int per_row = sh.cg / V, count = sh.s * per_row;
   const int col = (threadIdx.x % per_row) * V, row0 = threadIdx.x / per_row, step = blockDim.x / per_row;
   const T* xg = x + n * rx.sample + (int64_t)g * sh.cg + col;
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(1024) group_norm_held_backward_kernel(
       hd[j] = *reinterpret_cast<const Pack<T, V>*>(dyg + (row0 + j * step) * rdy.row);
     }
   }
-  const float mean = mean_in[blockIdx.x], rstd = rstd_in[blockIdx.x];
+  const float mean = mean_in[at], rstd = rstd_in[at];
   float ga[V], be[V], sb[V], sg[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(kThreads) group_norm_grad_sums_kernel(
   }
 }
 
-// Blocks 0 .. n * groups - 1: a (sample, group), group_sums = (mean(gamma dz), mean(gamma dz xh)).
+// Blocks 0 .. group_blocks - 1: (sample, group)s in turn, group_sums = (mean(gamma dz), mean(gamma dz xh)).
 // The blocks behind them: 8 columns of d_beta | d_gamma each, 32 threads a column.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) group_norm_fold_kernel(
@@ -409,20 +409,22 @@ __global__ void __launch_bounds__(kThreads) group_norm_fold_kernel(
   __shared__ double lds[32][9];
   if ((int)blockIdx.x < group_blocks) {
     __shared__ double2 waves[kThreads / 64];
-    const int n = blockIdx.x / sh.groups, c0 = (blockIdx.x % sh.groups) * sh.cg;
-    const float* p = partial + (int64_t)n * chunks * 2 * sh.c;
-    double2 t = make_double2(0, 0);
     const int items = chunks * sh.cg;
+    for (int at = blockIdx.x; at < sh.n * sh.groups; at += group_blocks) {
+      const int n = at / sh.groups, c0 = (at % sh.groups) * sh.cg;
+      const float* p = partial + (int64_t)n * chunks * 2 * sh.c;
+      double2 t = make_double2(0, 0);
 #pragma unroll 4
-    for (int j = threadIdx.x; j < items; j += kThreads) {
-      const int chunk = j / sh.cg, c = c0 + j % sh.cg;
-      const double ga = gamma ? load_param<T>(gamma, sh.param_f32, c) : 1.f;
-      t.x += ga * p[(int64_t)(2 * chunk) * sh.c + c];
-      t.y += ga * p[(int64_t)(2 * chunk + 1) * sh.c + c];
+      for (int j = threadIdx.x; j < items; j += kThreads) {
+        const int chunk = j / sh.cg, c = c0 + j % sh.cg;
+        const double ga = gamma ? load_param<T>(gamma, sh.param_f32, c) : 1.f;
+        t.x += ga * p[(int64_t)(2 * chunk) * sh.c + c];
+        t.y += ga * p[(int64_t)(2 * chunk + 1) * sh.c + c];
+      }
+      t = block_sum(t, waves);
+      const double inv = 1.0 / ((double)sh.s * sh.cg);
+      if (threadIdx.x == 0) group_sums[at] = make_float2((float)(t.x * inv), (float)(t.y * inv));
     }
-    t = block_sum(t, waves);
-    const double inv = 1.0 / ((double)sh.s * sh.cg);
-    if (threadIdx.x == 0) group_sums[blockIdx.x] = make_float2((float)(t.x * inv), (float)(t.y * inv));
     return;
   }
   const int col = (blockIdx.x - group_blocks) * 8 + (threadIdx.x & 7), l = threadIdx.x >> 3;
@@ -564,7 +566,8 @@ void backward_chunks(const PsGroupNormDesc& d, const Plan& p, const void* x, con
   float* partial = reinterpret_cast<float*>(group_sums + (size_t)d.samples * d.groups);
   group_norm_grad_sums_kernel<T, V><<<grid, kThreads, 0, st>>>(sh, p.rows, (const T*)x, rx, (const T*)dy, rdy, gamma,
                                                                beta, mean, rstd, partial);
-  const int group_blocks = d.samples * d.groups;
+  // a launch holds 2^32 threads, a batch up to 2^29 groups
+  const int group_blocks = d.samples * d.groups < 1 << 20 ? d.samples * d.groups : 1 << 20;
   group_norm_fold_kernel<T><<<group_blocks + (2 * d.channels + 7) / 8, kThreads, 0, st>>>(
       sh, p.chunks, group_blocks, partial, gamma, group_sums, d_gamma, d_beta);
   group_norm_grad_apply_kernel<T, V><<<grid, kThreads, 0, st>>>(sh, p.rows, (const T*)x, rx, (const T*)dy, rdy, gamma,
@@ -579,7 +582,7 @@ void forward_typed(const PsGroupNormDesc& d, const void* x, const void* gamma, c
   if (p.held) {
     const Shape sh = shape_of(d);
     const Rows rx = {d.x_sample_stride, d.x_row_stride};
-    const unsigned grid = (unsigned)(d.samples * d.groups);
+    const dim3 grid(d.groups, d.samples);
     if (p.held <= 2)
       group_norm_held_forward_kernel<T, V, 2><<<grid, p.threads, 0, st>>>(sh, (const T*)x, rx, gamma, beta, (T*)y, mean, rstd);
     else
@@ -600,7 +603,7 @@ void backward_typed(const PsGroupNormDesc& d, const void* x, const void* dy, con
   if (p.held) {
     const Shape sh = shape_of(d);
     const Rows rx = {d.x_sample_stride, d.x_row_stride}, rdy = {d.dy_sample_stride, d.dy_row_stride};
-    const unsigned grid = (unsigned)(d.samples * d.groups);
+    const dim3 grid(d.groups, d.samples);
     const size_t lds = (size_t)p.threads * V * 2 * sizeof(float);   // threads / (cg / V) rows of 2 cg floats
     float* partial = reinterpret_cast<float*>(workspace);
     if (p.held <= 2)
@@ -625,7 +628,7 @@ bool desc_ok(const PsGroupNormDesc* d) {
 }
 int unsupported(const PsGroupNormDesc& d) {
   return d.channels > 8192 || d.samples > 65535 || (int64_t)d.rows * d.channels >= (int64_t)1 << 31 ||
-         (int64_t)d.samples * d.groups > (1 << 24) || d.dtype < PS_DTYPE_F32 || d.dtype > PS_DTYPE_F16 ||
+         d.dtype < PS_DTYPE_F32 || d.dtype > PS_DTYPE_F16 ||
          d.activation < PS_ACT_NONE || d.activation > PS_ACT_SIGMOID;
 }
 

@@ -281,3 +281,13 @@ def test_group_norm_workspace_of_the_longest_samples(lib):
                 x_sample_stride=0, x_row_stride=1, dy_sample_stride=0, dy_row_stride=1)), b) for r in (rows, 1 << 30)
                 for b in (0, 1)]
             assert 0 < size[0] <= 2 * size[2] and 0 < size[1] <= 2 * size[3], (rows, size)
+
+
+def test_group_norm_takes_every_number_of_groups(lib):
+    """samples and channels at their limits with one channel a group: no limit of its own on their product."""
+    from pixelsplat_amd.ops import _lib
+    d = _lib.PsGroupNormDesc(samples=65535, rows=1, channels=8192, groups=8192, dtype=1, activation=0, param_f32=1, eps=1e-5,
+                             x_sample_stride=8192, x_row_stride=8192, dy_sample_stride=8192, dy_row_stride=8192)
+    # (mean, rstd)'s sums of every group at least, and of the gradient besides those of every channel
+    assert lib.ps_group_norm_workspace_bytes(C.byref(d), 0) >= 16 * 65535 * 8192
+    assert lib.ps_group_norm_workspace_bytes(C.byref(d), 1) >= 16 * 65535 * 8192

@@ -71,3 +71,11 @@ def test_sums_of_long_samples(gpu_device, c, groups, dtype):
     dw1 = torch.autograd.grad(group_norm(x, groups, w, b), w, x.detach())[0]      # xh = x rstd: terms of rstd
     want = n / math.sqrt(1 + 1e-5)
     assert ((dw1.double() - want).abs() <= 264 * R.U * want).all(), (dw1.double() - want).abs().max().item() / want / R.U
+
+
+@pytest.mark.parametrize("shape,groups", [((65535, 2, 512), 512), ((32800, 1, 8192), 512)], ids=str)
+def test_more_groups_than_a_launch_has_blocks(gpu_device, shape, groups):
+    """2^24 (sample, group)s and more: one channel each (chunks of rows), and 32 bytes each (one launch)."""
+    from tests.test_ops_group_norm_gpu import check, make
+
+    check(*make(gpu_device, shape, torch.bfloat16, torch.float32, seed=9), groups, "none")
