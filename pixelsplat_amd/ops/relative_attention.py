@@ -16,10 +16,15 @@ def relative_buckets(grid: tuple[int, int], buckets_per_axis: int = 32, max_dist
     buckets_per_axis / 4, then logarithmically wider ones that reach max_distance, the last holding all that is
     farther.  The two axes' buckets are combined row-major; an axis of one token has one bucket, so a 1 x n grid is a
     sequence with buckets_per_axis buckets.  The number of buckets is relative_bucket_count(grid, buckets_per_axis)."""
-    gh, gw = _grid(grid)
-    columns = 1 if gw == 1 else buckets_per_axis
-    rows, cols = (_axis(n, buckets_per_axis, max_distance) for n in (gh, gw))
-    return (rows[:, None] * columns + cols[None]).int().to(device)
+    columns = 1 if _grid(grid)[1] == 1 else buckets_per_axis
+    return _map(grid, buckets_per_axis, max_distance, columns, device)
+
+
+def _map(grid: tuple[int, int], buckets: int, max_distance: int, columns: int, device) -> Tensor:
+    # an ordinary tensor also where it is asked for in inference mode: training saves it for its backward pass
+    with torch.inference_mode(False):
+        rows, cols = (_axis(n, buckets, max_distance) for n in _grid(grid))
+        return (rows[:, None] * columns + cols[None]).int().to(device)
 
 
 def _axis(n: int, buckets: int, max_distance: int) -> Tensor:
@@ -79,8 +84,7 @@ class RelativePositionBias(nn.Module):
     def buckets(self, grid: tuple[int, int], device) -> Tensor:
         key = (*grid, torch.device(device))
         if key not in self._maps:
-            rows, cols = (_axis(n, self.buckets_per_axis, self.max_distance) for n in _grid(grid))
-            self._maps[key] = (rows[:, None] * self.buckets_per_axis + cols[None]).int().to(device)
+            self._maps[key] = _map(grid, self.buckets_per_axis, self.max_distance, self.buckets_per_axis, device)
         return self._maps[key]
 
     def matrix(self, grid: tuple[int, int]) -> Tensor:

@@ -291,3 +291,16 @@ def test_group_norm_takes_every_number_of_groups(lib):
     # (mean, rstd)'s sums of every group at least, and of the gradient besides those of every channel
     assert lib.ps_group_norm_workspace_bytes(C.byref(d), 0) >= 16 * 65535 * 8192
     assert lib.ps_group_norm_workspace_bytes(C.byref(d), 1) >= 16 * 65535 * 8192
+
+
+def test_bucket_maps_are_no_inference_tensors():
+    """A map made by a validation pass is what training saves for its backward pass later."""
+    from pixelsplat_amd.ops import RelativePositionBias, relative_buckets
+    net = RelativePositionBias(2, 8)
+    with torch.inference_mode():
+        made = net.buckets((3, 4), "cpu"), relative_buckets((3, 4), 8)
+    assert net.buckets((3, 4), "cpu") is made[0] and torch.equal(*made)
+    for t in made:
+        assert not t.is_inference()
+    net.matrix((3, 4)).sum().backward()
+    assert net.table.grad is not None
