@@ -349,9 +349,16 @@ Tensor token_rows(const Tensor& t, int64_t pad) {
   // copied token-major, as a packed projection would lay it out
   return ok ? t : t.transpose(1, 2).clone(at::MemoryFormat::Contiguous).transpose(1, 2);
 }
-Tensor token_major(const Tensor& like) {
-  return at::empty({like.size(0), like.size(2), like.size(1), like.size(3)}, like.options()).transpose(1, 2);
+// The first `dim` columns of a token-major [batch, heads, tokens, like's width].  No view of another tensor: autograd would
+// refuse to change a result in place that a function returns as a view.
+Tensor token_major(const Tensor& like, int64_t dim) {
+  const int64_t h = like.size(1), n = like.size(2), d = like.size(3);
+  const std::vector<int64_t> sizes = {like.size(0), h, n, dim}, strides = {n * h * d, d, h * d, 1};
+  if (dim == d) return at::empty_strided(sizes, strides, like.options());
+  const Tensor room = at::empty({like.numel()}, like.options());
+  return at::empty({0}, like.options()).set_(room.storage(), 0, sizes, strides);
 }
+Tensor token_major(const Tensor& like) { return token_major(like, like.size(3)); }
 void strides_of(const Tensor& t, int64_t* s) {
   for (int i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : vec_of(t);
 }
@@ -374,12 +381,13 @@ PsRelativeAttentionDesc attention_desc(const Tensor& q, const Tensor& k, const T
 
 struct Kept { Tensor out32, stats, bias; };
 
+// dim: of the result, whose rows are as wide as q's
 Tensor attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& buckets,
-                         const Tensor& mask, double scale, int64_t start, bool keep, Kept& kept) {
+                         const Tensor& mask, double scale, int64_t start, int64_t dim, bool keep, Kept& kept) {
   const PsRelativeAttentionDesc d = attention_desc(q, k, v, table, buckets, mask, scale, start, Tensor());
   const size_t size = ps_relative_attention_workspace_bytes(&d, 0);
   if (size == 0) throw std::runtime_error("relative_attention: unsupported configuration (see its limits)");
-  Tensor out = token_major(q);
+  Tensor out = token_major(q, dim);
   const auto fp32 = q.options().dtype(at::kFloat);
   kept.bias = at::empty({q.size(1), buckets.numel()}, fp32);
   if (keep) {
@@ -410,9 +418,9 @@ struct RelativeAttention : torch::autograd::Function<RelativeAttention> {
     const Tensor q = token_rows(q0.detach(), pad), k = token_rows(k0.detach(), pad), v = token_rows(v0.detach(), pad);
     const Tensor table = plain(table0);
     Kept kept;
-    Tensor out = attention_forward(q, k, v, table, buckets, mask, scale, start, true, kept);
+    Tensor out = attention_forward(q, k, v, table, buckets, mask, scale, start, q0.size(3), true, kept);
     ctx->save_for_backward({q, k, v, table, buckets, mask, kept.out32.defined() ? kept.out32 : out, kept.stats, kept.bias});
-    return pad ? out.narrow(3, 0, q0.size(3)) : out;
+    return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("relative_attention");
@@ -487,9 +495,8 @@ Tensor relative_attention(const Tensor& q, const Tensor& k, const Tensor& v, con
   if (q.numel() == 0) return token_major(q);
   const int64_t vec = vec_of(q), pad = (vec - dim % vec) % vec;
   Kept kept;
-  Tensor out = attention_forward(token_rows(q, pad), token_rows(k, pad), token_rows(v, pad), table.contiguous(), buckets, mask,
-                                 scale, start, false, kept);
-  return pad ? out.narrow(3, 0, dim) : out;
+  return attention_forward(token_rows(q, pad), token_rows(k, pad), token_rows(v, pad), table.contiguous(), buckets, mask, scale,
+                           start, dim, false, kept);
 }
 
 }  // namespace

@@ -61,7 +61,8 @@ def relative_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, buckets: 
     table [n, heads] in q's type or fp32; buckets [2 gh - 1, 2 gw - 1] int32 (relative_buckets, or any map of offsets;
     its shape names the grid; an entry outside 0 .. n - 1 is an offset without bias).  key_mask [batch, gh gw] bool,
     True for a key that is there; the values of masked keys do not matter, NaN included, and a row without keys is
-    zero.  scale: dim ** -0.5 by default.  Returns [batch, heads, queries, dim], token-major in memory.
+    zero.  scale: dim ** -0.5 by default.  Returns [batch, heads, queries, dim], token-major in memory; it may be changed
+    in place (in fp32 not before its backward pass, which reads it).
 
     dim <= 128, at most 2^20 keys, gw <= 512 on grids of more than one row.  Differentiable once in q, k, v and table;
     the gradient of the table is summed over the batch.  16-bit types accumulate in fp32; the
