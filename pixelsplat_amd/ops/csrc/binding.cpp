@@ -6,6 +6,7 @@
 // RuntimeError, raised before anything is allocated or launched.
 #include <ATen/ATen.h>
 #include <ATen/TensorUtils.h>
+#include <ATen/autocast_mode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -57,6 +58,13 @@ void check_device(const char* op, const Tensor& first, std::initializer_list<std
   for (const auto& o : others)
     if (o.second->defined() && o.second->device() != first.device())
       throw std::runtime_error(text(op, ": ", o.first, " is on ", o.second->device(), ", the input on ", first.device()));
+}
+
+// Under autocast the tensors of products take its type, as those of torch's own products do.  (The norm's and the
+// attention table's parameters may be fp32 beside 16-bit tensors and stay what they are.)
+Tensor cast(const Tensor& t) {
+  return t.defined() && at::autocast::is_autocast_enabled(at::kCUDA)
+             ? at::autocast::cached_cast(at::autocast::get_autocast_dtype(at::kCUDA), t, at::kCUDA) : t;
 }
 
 void check_status(const char* what, int rc) {
@@ -312,9 +320,10 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
   }
 };
 
-Tensor gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const std::optional<Tensor>& b_gate,
+Tensor gated_linear(const Tensor& x0, const Tensor& w_gate0, const Tensor& w_up0, const std::optional<Tensor>& b_gate,
                     const std::optional<Tensor>& b_up, int64_t act) {
-  const Tensor bg = b_gate.value_or(Tensor()), bu = b_up.value_or(Tensor());
+  const Tensor x = cast(x0), w_gate = cast(w_gate0), w_up = cast(w_up0), bg = cast(b_gate.value_or(Tensor())),
+               bu = cast(b_up.value_or(Tensor()));
   check_dtype("gated_linear", x);
   need_value(x.dim() >= 1 && w_gate.dim() == 2 && w_gate.sizes() == w_up.sizes() && w_gate.size(1) == x.size(-1),
              "gated_linear: x [..., dim] and two weights [hidden, dim], got ", shape(x), ", ", shape(w_gate), ", ", shape(w_up));
@@ -455,8 +464,9 @@ struct RelativeAttention : torch::autograd::Function<RelativeAttention> {
   }
 };
 
-Tensor relative_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& buckets0,
+Tensor relative_attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& table, const Tensor& buckets0,
                           const std::optional<Tensor>& key_mask, const std::optional<double>& scale0, int64_t start) {
+  const Tensor q = cast(q0), k = cast(k0), v = cast(v0);
   Tensor mask = key_mask.value_or(Tensor());
   check_dtype("relative_attention", q);
   need_value(q.dim() == 4 && k.dim() == 4 && k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(1) == q.size(1) &&

@@ -17,6 +17,6 @@ def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, b_gate: Optional[Tenso
     read in place when their rows are 16-byte aligned (dim a multiple of 8, or 4 in fp32), and copied otherwise.
     fp32 products are fp32 throughout; 16-bit ones accumulate in fp32 and round once.  Differentiable once in all five
     tensors: fp32 keeps both projections for it (8 bytes a hidden value), 16-bit types keep only their inputs.
-    Results repeat bit for bit."""
+    Under torch.autocast all five take its type, as in torch's own products.  Results repeat bit for bit."""
     act = _lib.activation_code("gated_linear", activation)
     return _lib.binding().gated_linear(x, w_gate, w_up, b_gate, b_up, act)

@@ -16,7 +16,7 @@ def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor] = None, bias
     torch.nn.functional.group_norm has them for channels-first tensors.  x: fp32, bf16 or fp16, any strides (a view
     [n, positions, c] with unit channel stride is read in place, anything else is copied first).  weight, bias [c]: x's
     type or fp32, each optional, both of one type.  activation: none, relu, silu, gelu (exact) or sigmoid.  The result
-    is contiguous.  Differentiable once in x, weight and bias; results repeat bit for bit."""
+    is contiguous, in x's type under torch.autocast too.  Differentiable once in x, weight and bias; results repeat bit for bit."""
     act = _lib.activation_code("group_norm", activation)
     return _lib.binding().group_norm(x, num_groups, weight, bias, eps, act)
 

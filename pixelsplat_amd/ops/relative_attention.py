@@ -64,6 +64,8 @@ def relative_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, buckets: 
     zero.  scale: dim ** -0.5 by default.  Returns [batch, heads, queries, dim], token-major in memory; it may be changed
     in place (in fp32 not before its backward pass, which reads it).
 
+    Under torch.autocast q, k and v take its type, as in torch's own products; the table keeps its own.
+
     dim <= 128, at most 2^20 keys, gw <= 512 on grids of more than one row.  Differentiable once in q, k, v and table;
     the gradient of the table is summed over the batch.  16-bit types accumulate in fp32; the
     backward rounds probabilities and the logits' gradients to them for its products.  Results repeat bit for bit."""

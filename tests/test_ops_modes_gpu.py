@@ -55,3 +55,42 @@ def test_results_changed_in_place(gpu_device, dim, dtype):
     empty = packed[:0].detach().requires_grad_()
     q = empty[:, :, 0].transpose(1, 2)
     assert relative_attention(q, q, q, table, buckets).mul_(2).shape == (0, 2, 15, dim)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_autocast(gpu_device, dtype):
+    """Products take autocast's type, whatever their inputs and parameters are in; parameters' gradients come back in
+    theirs.  A block of fp32 parameters trains behind a norm (fp32 there) and behind a projection (16 bits)."""
+    from pixelsplat_amd.encoder import GatedFeedForward, Transformer
+    from pixelsplat_amd.ops import gated_linear, group_norm, relative_attention, relative_buckets
+
+    torch.manual_seed(2)
+    x, w, b = (torch.randn(s, device=gpu_device, requires_grad=True) for s in ((6, 32), (2, 48, 32), (2, 48)))
+    low = lambda t: t.detach().to(dtype).requires_grad_()  # noqa: E731
+    xs, ws, bs = low(x), low(w), low(b)
+    want = gated_linear(xs, *ws, *bs)
+    dy = torch.randn_like(want)
+    for given in (x, x.detach().to(dtype)):
+        with torch.autocast("cuda", dtype):
+            y = gated_linear(given, *w, *b)
+        assert torch.equal(y, want)
+        for got, ref in zip(torch.autograd.grad(y, (w, b), dy), torch.autograd.grad(want, (ws, bs), dy, retain_graph=True)):
+            assert got.dtype == torch.float32 and torch.equal(got, ref.float())
+    q, k, v = (torch.randn((2, 2, 15, 16), device=gpu_device) for _ in range(3))
+    table = torch.randn((64, 2), device=gpu_device, requires_grad=True)
+    buckets = relative_buckets((3, 5), 8, device=gpu_device)
+    want = relative_attention(q.to(dtype), k.to(dtype), v.to(dtype), table, buckets)
+    with torch.autocast("cuda", dtype):
+        assert torch.equal(relative_attention(q, k.to(dtype), v, table, buckets), want)
+        assert group_norm(x, 4).dtype == torch.float32
+        with torch.autocast("cuda", enabled=False), pytest.raises(ValueError, match="w_gate is"):
+            gated_linear(xs, *w)
+
+    net = torch.nn.Sequential(torch.nn.Linear(32, 32), GatedFeedForward(32, 48)).to(gpu_device)
+    block = Transformer(32, 1, 2, 16, 48, feed_forward_layer=GatedFeedForward, relative_buckets=8).to(gpu_device)
+    for f in (lambda: net(torch.randn((2, 20, 32), device=gpu_device)),
+              lambda: block(torch.randn((2, 20, 32), device=gpu_device), grid=(4, 5))):
+        with torch.autocast("cuda", dtype):
+            f().float().square().sum().backward()
+    for p in [*net.parameters(), *block.parameters()]:
+        assert p.grad.dtype == torch.float32 and torch.isfinite(p.grad).all() and p.grad.abs().sum() > 0
