@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import torch
 from torch import nn
+from torch.nn.modules import module as nn_module
 
 from ..ops import RelativePositionBias, gated_linear
 
@@ -51,6 +52,13 @@ class PreNorm(nn.Module):
         return self.fn(self.norm(x), **kwargs)
 
 
+def _hooked(module: nn.Module) -> bool:
+    """Whether a hook of any kind waits for a call of `module`, one on all modules included."""
+    return any(len(hooks) > 0 for owner, prefix in ((module, ""), (nn_module, "_global"))
+               for hooks in (getattr(owner, prefix + kind) for kind in (
+                   "_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")))
+
+
 class Attention(nn.Module):
     """relative_buckets > 0 (self-attention only): a learned bias on the tokens' offsets on a grid,
     relative_buckets logarithmic buckets an axis.  forward then takes the grid (rows, columns) of the
@@ -85,9 +93,9 @@ class Attention(nn.Module):
             k, v = self.to_kv(z).chunk(2, dim=-1)
         split = lambda t: t.reshape(t.shape[0], t.shape[1], self.heads, -1).transpose(1, 2)
         q, k, v = split(q), split(k), split(v)
-        if self.relative_bias is not None and len(self.attend._forward_hooks) == 0:
+        if self.relative_bias is not None and not _hooked(self.attend):
             out = self.relative_bias(q, k, v, grid, key_mask, self.scale).transpose(1, 2)
-        else:   # a hook on `attend` sees the attention weights
+        else:   # a hook on `attend` sees the logits, the attention weights or their gradients
             logits = torch.matmul(q, k.transpose(-1, -2)) * self.scale
             if grid is not None:
                 logits = logits + self.relative_bias.matrix(grid).to(logits.dtype)

@@ -304,3 +304,27 @@ def test_bucket_maps_are_no_inference_tensors():
         assert not t.is_inference()
     net.matrix((3, 4)).sum().backward()
     assert net.table.grad is not None
+
+
+def test_hooks_on_the_attention_weights_see_them():
+    """A hook of any kind on `attend`, or on all modules, takes the form that computes the weights (which needs no GPU)."""
+    from torch.nn.modules import module as M
+
+    from pixelsplat_amd.encoder import Attention
+    net = Attention(16, 2, 8, relative_buckets=8)
+    x, seen = torch.randn(1, 6, 16), []
+    for add in (net.attend.register_forward_hook, net.attend.register_forward_pre_hook,
+                net.attend.register_full_backward_hook, net.attend.register_full_backward_pre_hook,
+                M.register_module_forward_hook, M.register_module_forward_pre_hook, M.register_module_full_backward_hook,
+                M.register_module_full_backward_pre_hook):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            net(x, grid=(2, 3))
+        handle = add(lambda module, *tensors: seen.append(module))
+        try:
+            net(x, grid=(2, 3)).sum().backward()
+        finally:
+            handle.remove()
+        assert net.attend in seen, add
+        seen.clear()
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        net(x, grid=(2, 3))
