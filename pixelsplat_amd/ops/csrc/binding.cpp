@@ -394,7 +394,7 @@ struct Kept { Tensor out32, stats, bias; };
 Tensor attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& buckets,
                          const Tensor& mask, double scale, int64_t start, int64_t dim, bool keep, Kept& kept) {
   const PsRelativeAttentionDesc d = attention_desc(q, k, v, table, buckets, mask, scale, start, Tensor());
-  const size_t size = ps_relative_attention_workspace_bytes(&d, 0);
+  const size_t size = ps_relative_attention_workspace_bytes(&d, PS_FORWARD);
   if (size == 0) throw std::runtime_error("relative_attention: unsupported configuration (see its limits)");
   Tensor out = token_major(q, dim);
   const auto fp32 = q.options().dtype(at::kFloat);
@@ -451,7 +451,7 @@ struct RelativeAttention : torch::autograd::Function<RelativeAttention> {
     const Tensor dout = token_rows(grads[0], q.size(3) - dim);
     const PsRelativeAttentionDesc d = attention_desc(q, k, v, table, buckets, mask, ctx->saved_data["scale"].toDouble(),
                                                      ctx->saved_data["start"].toInt(), dout);
-    const size_t size = ps_relative_attention_workspace_bytes(&d, 1);
+    const size_t size = ps_relative_attention_workspace_bytes(&d, dtable.defined() ? PS_BACKWARD : PS_BACKWARD_NO_TABLE);
     const Tensor ws = bytes(size, q);
     check_status("ps_relative_attention_backward",
                  ps_relative_attention_backward(&d, ptr(q), ptr(k), ptr(v), (const uint8_t*)ptr(mask),

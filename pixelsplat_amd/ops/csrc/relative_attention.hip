@@ -925,7 +925,8 @@ struct Plan {
   size_t delta, diag_rows, d_offsets, part_q, part_k, part_v, backward_total;
 };
 
-Plan plan(const PsRelativeAttentionDesc& d, bool training) {
+// table: its gradient is wanted, whose sums are all that grows with queries times keys
+Plan plan(const PsRelativeAttentionDesc& d, bool training, bool table = false) {
   Plan p = {};
   const int nk = d.grid_h * d.grid_w, e = d.dtype == PS_DTYPE_F32 ? 4 : 2;
   p.rows = e == 2 ? 64 : 32;
@@ -961,8 +962,10 @@ Plan plan(const PsRelativeAttentionDesc& d, bool training) {
   p.forward_total = at + 256;
   at = 0;
   p.delta = take(sizeof(float) * bh * p.nq_pad);
-  p.diag_rows = take(sizeof(float) * bh * (p.nq_pad / 32) * p.dq.splits * p.sums * p.diag_pitch);
-  p.d_offsets = take(sizeof(double) * d.heads * p.offsets);
+  if (table) {
+    p.diag_rows = take(sizeof(float) * bh * (p.nq_pad / 32) * p.dq.splits * p.sums * p.diag_pitch);
+    p.d_offsets = take(sizeof(double) * d.heads * p.offsets);
+  }
   if (p.dq.splits > 1) p.part_q = take(sizeof(float) * p.dq.splits * rows * d.dim);
   if (p.dkv.splits > 1) {
     p.part_k = take(sizeof(float) * p.dkv.splits * bh * nk * d.dim);
@@ -1114,9 +1117,9 @@ using namespace ps;
 
 extern "C" {
 
-size_t ps_relative_attention_workspace_bytes(const PsRelativeAttentionDesc* d, int32_t backward) {
+size_t ps_relative_attention_workspace_bytes(const PsRelativeAttentionDesc* d, int32_t pass) {
   if (check(d)) return 0;
-  if (backward) return plan(*d, true).backward_total;
+  if (pass != PS_FORWARD) return plan(*d, true, pass != PS_BACKWARD_NO_TABLE).backward_total;
   const size_t a = plan(*d, false).forward_total, b = plan(*d, true).forward_total;
   return a > b ? a : b;
 }
@@ -1132,7 +1135,7 @@ int ps_relative_attention_forward(const PsRelativeAttentionDesc* d, const void* 
   if (!bucket_map || !table || !out || !aligned16(out) || !bias || !workspace || !aligned16(workspace) ||
       (out_f32 && !aligned16(out_f32)))
     return PS_ERR_BAD_ARG;
-  if (workspace_bytes < ps_relative_attention_workspace_bytes(d, 0)) return PS_ERR_WORKSPACE;
+  if (workspace_bytes < ps_relative_attention_workspace_bytes(d, PS_FORWARD)) return PS_ERR_WORKSPACE;
   const Plan p = plan(*d, stats != nullptr);
   Args a = args_of(*d, p);
   a.q = q; a.k = k; a.v = v; a.mask = key_mask; a.bias = bias;
@@ -1160,8 +1163,8 @@ int ps_relative_attention_backward(const PsRelativeAttentionDesc* d, const void*
   if (int rc = check_rows(*d, d_out, d->do_strides)) return rc;
   if (!bucket_map || !bias || !out_f32 || !stats || !workspace || !aligned16(workspace)) return PS_ERR_BAD_ARG;
   if (!aligned16(dq) || !aligned16(dk) || !aligned16(dv)) return PS_ERR_BAD_ARG;
-  if (workspace_bytes < ps_relative_attention_workspace_bytes(d, 1)) return PS_ERR_WORKSPACE;
-  const Plan p = plan(*d, true);
+  const Plan p = plan(*d, true, d_table != nullptr);
+  if (workspace_bytes < p.backward_total) return PS_ERR_WORKSPACE;
   Args a = args_of(*d, p);
   char* ws = (char*)workspace;
   a.q = q; a.k = k; a.v = v; a.mask = key_mask; a.bias = bias; a.dout = d_out;

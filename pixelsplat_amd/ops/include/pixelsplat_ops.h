@@ -93,7 +93,10 @@ typedef struct PsRelativeAttentionDesc {
   int64_t q_strides[3], k_strides[3], v_strides[3], do_strides[3];
   int64_t mask_stride; /* of a batch element */
 } PsRelativeAttentionDesc;
-size_t ps_relative_attention_workspace_bytes(const PsRelativeAttentionDesc* desc, int32_t backward);
+#define PS_FORWARD 0
+#define PS_BACKWARD 1          /* with d_table: grows with queries x keys */
+#define PS_BACKWARD_NO_TABLE 2 /* d_table is NULL */
+size_t ps_relative_attention_workspace_bytes(const PsRelativeAttentionDesc* desc, int32_t pass);
 int ps_relative_attention_forward(const PsRelativeAttentionDesc* desc, const void* q, const void* k, const void* v,
                                   const uint8_t* key_mask, const int32_t* bucket_map, const void* table, void* out,
                                   float* out_f32, float* stats, float* bias, void* workspace, size_t workspace_bytes,

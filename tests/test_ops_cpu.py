@@ -328,3 +328,19 @@ def test_hooks_on_the_attention_weights_see_them():
         seen.clear()
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         net(x, grid=(2, 3))
+
+
+def test_attention_workspace_without_the_tables_gradient(lib):
+    """Where the table is frozen, nothing grows with queries times keys: 16 times the tokens take 16 times the bytes."""
+    from pixelsplat_amd.ops import _lib
+
+    def size(side, what):
+        s = (C.c_int64 * 3)(side * side * 64, 64, 64)
+        return lib.ps_relative_attention_workspace_bytes(C.byref(_lib.PsRelativeAttentionDesc(
+            batch=2, heads=1, queries=side * side, query_start=0, grid_h=side, grid_w=side, dim=64, dtype=1, buckets=5,
+            table_f32=0, scale=0.3, reserved=0, q_strides=s, k_strides=s, v_strides=s, do_strides=s, mask_stride=0)), what)
+
+    for side in (32, 64, 128, 512):
+        assert 0 < size(side, 2) <= 2 * side * side * 64 * 4 * 3 * 16 + (1 << 20), side      # parts of up to 16 splits
+        assert size(side, 2) < size(side, 1)
+    assert size(512, 2) <= 16 * size(128, 2) and size(512, 1) > 128 * size(128, 1)

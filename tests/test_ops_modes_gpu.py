@@ -94,3 +94,23 @@ def test_autocast(gpu_device, dtype):
             f().float().square().sum().backward()
     for p in [*net.parameters(), *block.parameters()]:
         assert p.grad.dtype == torch.float32 and torch.isfinite(p.grad).all() and p.grad.abs().sum() > 0
+
+
+def test_a_frozen_table_takes_no_room_for_its_gradient(gpu_device):
+    """128 x 128 tokens: 2 x 128^4 / 8 bytes of sums for the table's gradient, none of them where it is not wanted."""
+    from pixelsplat_amd.ops import relative_attention, relative_buckets
+
+    buckets = relative_buckets((128, 128), 8, device=gpu_device)
+    q = torch.randn((1, 1, 16384, 16), device=gpu_device).bfloat16().requires_grad_()
+    table = torch.randn((64, 1), device=gpu_device)
+    want = None
+    for wanted in (True, False):
+        y = relative_attention(q, q, q, table.requires_grad_(wanted), buckets)
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        got = torch.autograd.grad(y, q, torch.ones_like(y))[0] if not wanted else \
+            torch.autograd.grad(y, (q, table), torch.ones_like(y))[0]
+        used = torch.cuda.max_memory_allocated() - before
+        assert used > 2 * 16384 ** 2 // 8 if wanted else used < 32 << 20, (wanted, used)
+        assert want is None or torch.equal(got, want)
+        want = got
