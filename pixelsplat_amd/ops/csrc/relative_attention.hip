@@ -846,44 +846,85 @@ __global__ void __launch_bounds__(256) join_gradients_kernel(Gradients a) {
 }
 
 constexpr int kJoinHeads = 8, kJoinList = 8192;
+constexpr int kJoinLists = 512;          // of the longest map: a grid of 2^20 tokens has less than 2^22 offsets
+
+// ranges[i] = lowest and highest bucket of entries kJoinList i .. of the map
+__global__ void __launch_bounds__(256) bucket_ranges_kernel(int offsets, const int32_t* __restrict__ map, int2* __restrict__ ranges) {
+  __shared__ int2 lds[4];
+  const int end = min((int)(blockIdx.x + 1) * kJoinList, offsets);
+  int lo = INT32_MAX, hi = INT32_MIN;
+  for (int i = blockIdx.x * kJoinList + threadIdx.x; i < end; i += 256) {
+    lo = min(lo, map[i]);
+    hi = max(hi, map[i]);
+  }
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) {
+    lo = min(lo, __shfl_xor(lo, m));
+    hi = max(hi, __shfl_xor(hi, m));
+  }
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = make_int2(lo, hi);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 4; ++w) {
+      lo = min(lo, lds[w].x);
+      hi = max(hi, lds[w].y);
+    }
+    ranges[blockIdx.x] = make_int2(lo, hi);
+  }
+}
 
 // d_table[bucket][head]: a block a bucket and 8 heads.  It lists the offsets of its bucket, in order -- kJoinList entries
-// of the map at a time, a run of them a wave -- then 32 threads a head take the list's entries.
+// of the map at a time, a run of them a wave -- then 32 threads a head take the list's entries.  With `ranges` it passes over
+// runs of entries that cannot hold its bucket.
 template <typename T>
 __global__ void __launch_bounds__(256) join_offsets_kernel(int heads, int offsets, int buckets, const int32_t* __restrict__ map,
-                                                           const double* __restrict__ d_offsets, void* __restrict__ d_table,
-                                                           int table_f32) {
+                                                           const int2* __restrict__ ranges, const double* __restrict__ d_offsets,
+                                                           void* __restrict__ d_table, int table_f32) {
   constexpr int kRun = kJoinList / 4;
   __shared__ int list[4][kRun];
   __shared__ int found[4];
   __shared__ double lds[32][kJoinHeads + 1];
-  const int bucket = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  __shared__ uint64_t held[kJoinLists / 64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int j = threadIdx.x & (kJoinHeads - 1), h = blockIdx.y * kJoinHeads + j, part = threadIdx.x / kJoinHeads;
   const double* of_h = d_offsets + (int64_t)min(h, heads - 1) * offsets;
-  double t = 0;
-  for (int base = 0; base < offsets; base += kJoinList) {
-    int mine[kRun / 64], n = 0;
-    const int from = base + wave * kRun + lane;
-#pragma unroll
-    for (int i = 0; i < kRun / 64; ++i) mine[i] = from + i * 64 < offsets ? map[from + i * 64] : -1;
-#pragma unroll
-    for (int i = 0; i < kRun / 64; ++i) {
-      const uint64_t hits = __ballot(mine[i] == bucket);
-      if (mine[i] == bucket) list[wave][n + __popcll(hits & ((1ull << lane) - 1))] = from + i * 64;
-      n += __popcll(hits);
+  for (int bucket = blockIdx.x; bucket < buckets; bucket += gridDim.x) {      // a launch has no 2^24 blocks of 256
+    if (ranges) {
+      for (int i = threadIdx.x; i < kJoinLists; i += 256) {
+        const int2 r = i * kJoinList < offsets ? ranges[i] : make_int2(1, 0);
+        const uint64_t hits = __ballot(r.x <= bucket && bucket <= r.y);
+        if (lane == 0) held[i >> 6] = hits;
+      }
+      __syncthreads();
     }
-    if (lane == 0) found[wave] = n;
-    __syncthreads();
-    for (int w = 0; w < 4; ++w)
+    double t = 0;
+    for (int base = 0; base < offsets; base += kJoinList) {
+      const int at = base / kJoinList;
+      if (ranges && !((held[at >> 6] >> (at & 63)) & 1)) continue;
+      int mine[kRun / 64], n = 0;
+      const int from = base + wave * kRun + lane;
+#pragma unroll
+      for (int i = 0; i < kRun / 64; ++i) mine[i] = from + i * 64 < offsets ? map[from + i * 64] : -1;
+#pragma unroll
+      for (int i = 0; i < kRun / 64; ++i) {
+        const uint64_t hits = __ballot(mine[i] == bucket);
+        if (mine[i] == bucket) list[wave][n + __popcll(hits & ((1ull << lane) - 1))] = from + i * 64;
+        n += __popcll(hits);
+      }
+      if (lane == 0) found[wave] = n;
+      __syncthreads();
+      for (int w = 0; w < 4; ++w)
 #pragma unroll 4
-      for (int i = part; i < found[w]; i += 32) t += of_h[list[w][i]];
+        for (int i = part; i < found[w]; i += 32) t += of_h[list[w][i]];
+      __syncthreads();
+    }
+    lds[part][j] = t;
     __syncthreads();
-  }
-  lds[part][j] = t;
-  __syncthreads();
-  if (part == 0 && h < heads) {
-    for (int k = 1; k < 32; ++k) t += lds[k][j];
-    store_param<T>(d_table, table_f32, (int64_t)bucket * heads + h, (float)t);
+    if (part == 0 && h < heads) {
+      for (int k = 1; k < 32; ++k) t += lds[k][j];
+      store_param<T>(d_table, table_f32, (int64_t)bucket * heads + h, (float)t);
+    }
+    __syncthreads();
   }
 }
 
@@ -918,12 +959,20 @@ Split split_of(int64_t blocks, int want, int tiles) {
   return {count(tiles, per), per};
 }
 
+constexpr int64_t kManyReads = (int64_t)1 << 28;
+
 struct Plan {
   int waves, rows, nq_pad, window, window_b, sums, diag_pitch, offsets, dp;
   Split forward, dq, dkv;
   size_t part_o, part_ml, forward_total;
-  size_t delta, diag_rows, d_offsets, part_q, part_k, part_v, backward_total;
+  size_t delta, diag_rows, d_offsets, ranges, part_q, part_k, part_v, backward_total;
 };
+
+// Every bucket's block reads the whole map, unless a launch more tells it where its bucket cannot be.  The whole training
+// pass of 64 queries of 8 heads with a bucket for every offset, with it / without: 96 x 96 keys (2^30.3 reads) 239 / 529 us,
+// 256 x 256 (2^36) 1.8 / 18.3 ms; below 2^28 reads the join is 10 us of 100 - 170 and another launch takes 3.  A map whose
+// buckets lie anywhere gains nothing from it, and its join stays at buckets times offsets: 18.7 ms at 256 x 256.
+bool many_reads(const PsRelativeAttentionDesc& d, int offsets) { return (int64_t)d.buckets * offsets >= kManyReads; }
 
 // table: its gradient is wanted, whose sums are all that grows with queries times keys
 Plan plan(const PsRelativeAttentionDesc& d, bool training, bool table = false) {
@@ -965,6 +1014,7 @@ Plan plan(const PsRelativeAttentionDesc& d, bool training, bool table = false) {
   if (table) {
     p.diag_rows = take(sizeof(float) * bh * (p.nq_pad / 32) * p.dq.splits * p.sums * p.diag_pitch);
     p.d_offsets = take(sizeof(double) * d.heads * p.offsets);
+    if (many_reads(d, p.offsets)) p.ranges = take(sizeof(int2) * kJoinLists);
   }
   if (p.dq.splits > 1) p.part_q = take(sizeof(float) * p.dq.splits * rows * d.dim);
   if (p.dkv.splits > 1) {
@@ -1068,16 +1118,20 @@ int forward_typed(const PsRelativeAttentionDesc& d, Args a, const Plan& p, const
 }
 
 template <typename T>
-int backward_typed(const PsRelativeAttentionDesc& d, Args a, const Plan& p, const int32_t* map, void* d_table,
-                   double* d_offsets, hipStream_t st) {
+int backward_typed(const PsRelativeAttentionDesc& d, Args a, const Plan& p, const int32_t* map, void* d_table, char* ws,
+                   hipStream_t st) {
   const int rc = p.dp == 32 ? run_backward<T, 32>(a, p, d_table != nullptr, st)
                : p.dp == 64 ? run_backward<T, 64>(a, p, d_table != nullptr, st)
                             : run_backward<T, 128>(a, p, d_table != nullptr, st);
   if (rc || !d_table) return rc;
   a.splits = p.dq.splits;
+  double* d_offsets = (double*)(ws + p.d_offsets);
   join_diagonals_kernel<<<dim3((unsigned)count(p.offsets, 16), (unsigned)d.heads), 256, 0, st>>>(a, p.sums, d_offsets);
-  join_offsets_kernel<T><<<dim3((unsigned)d.buckets, (unsigned)count(d.heads, kJoinHeads)), 256, 0, st>>>(
-      d.heads, p.offsets, d.buckets, map, d_offsets, d_table, d.table_f32);
+  int2* ranges = many_reads(d, p.offsets) ? (int2*)(ws + p.ranges) : nullptr;
+  if (ranges) bucket_ranges_kernel<<<(unsigned)count(p.offsets, kJoinList), 256, 0, st>>>(p.offsets, map, ranges);
+  const unsigned blocks = (unsigned)(d.buckets < 1 << 20 ? d.buckets : 1 << 20);
+  join_offsets_kernel<T><<<dim3(blocks, (unsigned)count(d.heads, kJoinHeads)), 256, 0, st>>>(
+      d.heads, p.offsets, d.buckets, map, ranges, d_offsets, d_table, d.table_f32);
   return PS_OK;
 }
 
@@ -1172,13 +1226,12 @@ int ps_relative_attention_backward(const PsRelativeAttentionDesc* d, const void*
   a.diag_rows = (float*)(ws + p.diag_rows);
   a.part_q = (float*)(ws + p.part_q); a.part_k = (float*)(ws + p.part_k); a.part_v = (float*)(ws + p.part_v);
   a.dq = dq; a.dk = dk; a.dv = dv;
-  double* d_offsets = (double*)(ws + p.d_offsets);
   hipStream_t st = (hipStream_t)stream;
   int rc;
   switch (d->dtype) {
-    case PS_DTYPE_F32: rc = backward_typed<float>(*d, a, p, bucket_map, d_table, d_offsets, st); break;
-    case PS_DTYPE_BF16: rc = backward_typed<bf16>(*d, a, p, bucket_map, d_table, d_offsets, st); break;
-    default: rc = backward_typed<f16>(*d, a, p, bucket_map, d_table, d_offsets, st); break;
+    case PS_DTYPE_F32: rc = backward_typed<float>(*d, a, p, bucket_map, d_table, ws, st); break;
+    case PS_DTYPE_BF16: rc = backward_typed<bf16>(*d, a, p, bucket_map, d_table, ws, st); break;
+    default: rc = backward_typed<f16>(*d, a, p, bucket_map, d_table, ws, st); break;
   }
   return rc ? rc : hipGetLastError() == hipSuccess ? PS_OK : PS_ERR_LAUNCH;
 }
