@@ -18,7 +18,7 @@
 // What the backward needs of a and u: fp32 tensors keep both (8 bytes a hidden value, against 4 D flop at 150
 // TFLOP/s); 16-bit tensors compute them again (the products are 8 times as fast, and keeping them rounded to 16 bits
 // would put a second rounding into every gradient).  da and du are rounded to the tensors' type before they enter
-// their products, as h is before its own.
+// their products, as h is before its own; in fp16 they are first brought into its range (range_kernel).
 #include "mfma_tile.h"
 #include "pixelsplat_ops.h"
 
@@ -135,6 +135,7 @@ product_kernel(Product g, EP ep) {
   constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, kK = kSliceBytes / sizeof(T);
   constexpr int kA = BM * kSliceBytes, kB = BN * kSliceBytes;
   extern __shared__ __attribute__((aligned(16))) char lds[];    // 2 x (A | B)
+  if (ep.done()) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, hi = lane >> 5;
   const int wm = wave / WN, wn = wave % WN;
   // tiles of 8 rows of tiles at a time, column by column: neighbours share their operands in the die's L2
@@ -199,7 +200,10 @@ product_kernel(Product g, EP ep) {
 
 // ---- epilogues --------------------------------------------------------------------------------------------------
 // h, and (fp32 training) a and u
-struct StoreGated {
+struct NotDone {
+  __device__ __forceinline__ bool done() const { return false; }
+};
+struct StoreGated : NotDone {
   void* h;
   const void *bg, *bu;
   float *a, *u;           // NULL: not kept
@@ -241,6 +245,12 @@ struct StoreGated {
   }
 };
 
+template <typename T> constexpr bool kNarrow = false;     // a type whose exponents are fewer than fp32's
+template <> constexpr bool kNarrow<f16> = true;
+
+// fp16: what da and du are multiplied by before they are rounded, and its inverse; powers of two.
+struct Range { float scale, inverse; };
+
 // da and du (16-bit) from the recomputed projections; with biases, their column sums over the wave's rows.  dh comes
 // through LDS where it lies in whole aligned chunks; da takes its place there.
 struct StoreGatedGrad {
@@ -252,10 +262,15 @@ struct StoreGatedGrad {
   int ld;
   float* sums;            // [row parts][2][ld] or NULL
   int act;
+  float* peaks;           // fp16: the largest finite |da| and |du| of every wave
+  const Range* range;     // fp16, the second time: see range_kernel
+  __device__ __forceinline__ bool done() const { return range != nullptr && range->scale == 1.f; }
   template <typename TL>
   __device__ __forceinline__ void store(const floatx16 (&acc)[TL::TM][TL::TN], const TL& t, const Product& g) const {
     typedef typename TL::T T;
     typedef Staged<T, TL::BM, TL::BN / 2, TL::THREADS> St;
+    const float by = kNarrow<T> && range ? range->scale : 1.f;
+    float peak = 0.f;
     char *ta = t.lds, *tu = t.lds + St::kBytes;
     const int u0 = t.n0 / 2;
     if (dh_chunks) {
@@ -290,8 +305,15 @@ struct StoreGatedGrad {
               va = d * (acc[i][j + 1][r] + wu) * slope;
               vu = d * value;
             }
-            *St::at(ta, in, col) = from_f32<T>(va);
-            *St::at(tu, in, col) = from_f32<T>(vu);
+            if constexpr (kNarrow<T>) {
+              const float top = fmaxf(fabsf(va), fabsf(vu));
+              if (top < __builtin_inff()) peak = fmaxf(peak, top);
+              *St::at(ta, in, col) = from_f32<T>(va * by);
+              *St::at(tu, in, col) = from_f32<T>(vu * by);
+            } else {
+              *St::at(ta, in, col) = from_f32<T>(va);
+              *St::at(tu, in, col) = from_f32<T>(vu);
+            }
             sa += va;
             su += vu;
           }
@@ -305,6 +327,11 @@ struct StoreGatedGrad {
         }
       }
     });
+    if constexpr (kNarrow<T>) {
+#pragma unroll
+      for (int m = 32; m >= 1; m >>= 1) peak = fmaxf(peak, __shfl_xor(peak, m));
+      if (t.lane == 0) peaks[blockIdx.x * (TL::THREADS / 64) + (threadIdx.x >> 6)] = peak;
+    }
     __syncthreads();
     St::flush(ta, (T*)da, ld, t.m0, g.m, u0, ld);
     St::flush(tu, (T*)du, ld, t.m0, g.m, u0, ld);
@@ -312,15 +339,17 @@ struct StoreGatedGrad {
 };
 
 // the product itself, or this split's part of it in fp32
-struct StoreMatrix {
+struct StoreMatrix : NotDone {
   void* c[2];             // by blockIdx.z
   float* parts;           // [blockIdx.z][splits][m][n] or NULL
+  const Range* range;     // fp16: what its first operand was multiplied by
   template <typename TL>
   __device__ __forceinline__ void store(const floatx16 (&acc)[TL::TM][TL::TN], const TL& t, const Product& g) const {
     typedef typename TL::T T;
     typedef Staged<T, TL::BM, TL::BN, TL::THREADS> St;
     T* out = reinterpret_cast<T*>(blockIdx.z ? c[1] : c[0]);
     const bool staged = sizeof(T) == 2 && !parts;       // n is a multiple of 8
+    const float by = kNarrow<T> ? range->inverse : 1.f;
 #pragma unroll
     for (int j = 0; j < TL::TN; ++j) {
       const int in_col = (t.wn * TL::TN + j) * 32 + (t.lane & 31), col = t.n0 + in_col;
@@ -330,9 +359,10 @@ struct StoreMatrix {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int in = (t.wm * TL::TM + i) * 32 + result_row(r, t.lane >> 5), row = t.m0 + in;
-          if (staged) *St::at(t.lds, in, in_col) = from_f32<T>(acc[i][j][r]);
-          else if (row < g.m && parts) parts[(((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * g.m + row) * g.n + col] = acc[i][j][r];
-          else if (row < g.m) out[(int64_t)row * g.n + col] = from_f32<T>(acc[i][j][r]);
+          const float v = kNarrow<T> ? acc[i][j][r] * by : acc[i][j][r];
+          if (staged) *St::at(t.lds, in, in_col) = from_f32<T>(v);
+          else if (row < g.m && parts) parts[(((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * g.m + row) * g.n + col] = v;
+          else if (row < g.m) out[(int64_t)row * g.n + col] = from_f32<T>(v);
         }
     }
     if (staged) {
@@ -343,6 +373,28 @@ struct StoreMatrix {
 };
 
 // ---- small kernels ----------------------------------------------------------------------------------------------
+// fp16 holds less than the products it is an operand of: da = dh u act'(a) of 2^17 is infinite in it though dx is not, and
+// below 2^-14 it has few bits.  So da and du are computed twice where their largest value lies outside 2^-6 .. 65504, the
+// second time multiplied by the power of two that takes it to 2^14 .. 2^15; the products' results are divided by it.  Where it
+// lies inside (what is smaller is off by 2^-25 at most, 2^-19 of the largest), the second launch ends at once.  A scale a row
+// would do for dx, but rows are what dW sums over.  The training pass of 16384 x 1024 -> 4096: 1443 us without either, 1476 as it
+// is, 1871 where it computes them twice.
+__global__ void __launch_bounds__(1024) range_kernel(int64_t n, const float* __restrict__ peaks, Range* __restrict__ range) {
+  __shared__ float lds[16];
+  float peak = 0.f;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) peak = fmaxf(peak, peaks[i]);
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) peak = fmaxf(peak, __shfl_xor(peak, m));
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = peak;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) peak = fmaxf(peak, lds[w]);
+    int up = 0;
+    if (peak > 65504.f || (peak > 0.f && peak < 0.015625f)) up = max(-100, min(100, 14 - ilogbf(peak)));
+    *range = {ldexpf(1.f, up), ldexpf(1.f, -up)};
+  }
+}
+
 // fp32: da, du of the kept projections.  A block takes `rows` rows of 256 columns and leaves their column sums.
 __global__ void __launch_bounds__(256) gated_slope_kernel(int m, int n, int ld, int rows, int act, const float* __restrict__ a,
                                                           const float* __restrict__ u, const float* __restrict__ dh,
@@ -549,11 +601,11 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 struct BackwardPlan {
   int ld, sum_parts, slope_rows;
   Tiling again, dx, dw;
-  size_t da, du, sums, parts_x, parts_w, total;
+  size_t da, du, sums, peaks, range, parts_x, parts_w, total;
 };
 
 BackwardPlan backward_plan(const PsGatedLinearDesc& d) {
-  BackwardPlan p;
+  BackwardPlan p = {};
   const size_t e = d.dtype == PS_DTYPE_F32 ? 4 : 2;
   p.ld = pad8(d.hidden);
   p.again = tiling(d.dtype, d.rows, 2 * p.ld, d.dim, 1, 1, false);
@@ -567,6 +619,10 @@ BackwardPlan backward_plan(const PsGatedLinearDesc& d) {
   p.da = at; at += align256(e * d.rows * p.ld);
   p.du = at; at += align256(e * d.rows * p.ld);
   p.sums = at; at += align256(sizeof(float) * p.sum_parts * 2 * p.ld);
+  if (d.dtype == PS_DTYPE_F16) {
+    p.peaks = at; at += align256(sizeof(float) * 8 * p.again.tiles_m * (size_t)p.again.tiles_n);   // 8 waves a tile at most
+    p.range = at; at += align256(sizeof(Range));
+  }
   p.parts_x = at; at += p.dx.splits > 1 ? align256(sizeof(float) * p.dx.splits * (size_t)d.rows * d.dim) : 0;
   p.parts_w = at; at += p.dw.splits > 1 ? align256(sizeof(float) * 2 * p.dw.splits * (size_t)d.hidden * d.dim) : 0;
   p.total = at;
@@ -592,7 +648,7 @@ int forward_typed(const PsGatedLinearDesc& d, const void* x, const void* wg, con
   g.m = d.rows; g.n = d.hidden; g.k = d.dim; g.halves = 1;
   g.a.p[0] = x; g.a.ld = d.x_row_stride;
   g.b.p[0] = wg; g.b.p[1] = wu; g.b.ld = d.w_row_stride;
-  StoreGated ep = {h, bg, bu, a, u, d.activation};
+  StoreGated ep = {{}, h, bg, bu, a, u, d.activation};
   return launch_product<T, false, false, true>(g, tiling(d.dtype, d.rows, 2 * d.hidden, d.dim, 1, 1, false), ep, st);
 }
 
@@ -606,6 +662,7 @@ int backward_typed(const PsGatedLinearDesc& d, const void* x, const void* wg, co
   float* sums = dbg || dbu ? (float*)(ws + p.sums) : nullptr;
   float* parts_x = p.dx.splits > 1 ? (float*)(ws + p.parts_x) : nullptr;
   float* parts_w = p.dw.splits > 1 ? (float*)(ws + p.parts_w) : nullptr;
+  const Range* range = kNarrow<T> ? (const Range*)(ws + p.range) : nullptr;
   Finish f = {};
   if constexpr (sizeof(T) == 4) {
     const dim3 grid((unsigned)((p.ld + 255) / 256), (unsigned)p.sum_parts);
@@ -617,8 +674,14 @@ int backward_typed(const PsGatedLinearDesc& d, const void* x, const void* wg, co
     g.a.p[0] = x; g.a.ld = d.x_row_stride;
     g.b.p[0] = wg; g.b.p[1] = wu; g.b.ld = d.w_row_stride;
     const int chunks = d.hidden % 8 == 0 && d.dh_row_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(dh) & 15) == 0;
-    StoreGatedGrad ep = {dh, d.dh_row_stride, chunks, bg, bu, da, du, p.ld, sums, d.activation};
+    StoreGatedGrad ep = {dh, d.dh_row_stride, chunks, bg, bu, da, du, p.ld, sums, d.activation, (float*)(ws + p.peaks), nullptr};
     if (int rc = launch_product<T, false, false, true>(g, p.again, ep, st)) return rc;
+    if (kNarrow<T>) {
+      const int waves = p.again.bm == 256 ? 8 : p.again.bm == 128 ? 4 : 2;
+      range_kernel<<<1, 1024, 0, st>>>((int64_t)p.again.tiles_m * p.again.tiles_n * waves, ep.peaks, (Range*)range);
+      ep.range = range;
+      if (int rc = launch_product<T, false, false, true>(g, p.again, ep, st)) return rc;
+    }
   }
   auto join = [](const Tiling& t, int64_t count, const float* parts, int matrices, void* c0, void* c1) {
     Join j = {count, t.splits, matrices, (int)((count * matrices / 4 + 255) / 256), parts, {c0, c1}};
@@ -629,7 +692,7 @@ int backward_typed(const PsGatedLinearDesc& d, const void* x, const void* wg, co
     g.m = d.rows; g.n = d.dim; g.k = d.hidden; g.halves = 2;
     g.a.p[0] = da; g.a.p[1] = du; g.a.ld = p.ld;
     g.b.p[0] = wg; g.b.p[1] = wu; g.b.ld = d.w_row_stride;
-    StoreMatrix ep = {{dx, nullptr}, parts_x};
+    StoreMatrix ep = {{}, {dx, nullptr}, parts_x, range};
     if (int rc = launch_product<T, false, true, false>(g, p.dx, ep, st)) return rc;
     if (parts_x) f.join[0] = join(p.dx, (int64_t)d.rows * d.dim, parts_x, 1, dx, nullptr);
   }
@@ -639,7 +702,7 @@ int backward_typed(const PsGatedLinearDesc& d, const void* x, const void* wg, co
     g.m = d.hidden; g.n = d.dim; g.k = d.rows; g.halves = 1; g.first = dwg ? 0 : 1;
     g.a.p[0] = da; g.a.p[1] = du; g.a.ld = p.ld;
     g.b.p[0] = x; g.b.ld = d.x_row_stride;
-    StoreMatrix ep = {{dwg ? dwg : dwu, dwu}, parts_w};
+    StoreMatrix ep = {{}, {dwg ? dwg : dwu, dwu}, parts_w, range};
     if (int rc = launch_product<T, true, true, false>(g, p.dw, ep, st, products)) return rc;
     if (parts_w) f.join[1] = join(p.dw, (int64_t)d.hidden * d.dim, parts_w, products, dwg ? dwg : dwu, dwu);
   }

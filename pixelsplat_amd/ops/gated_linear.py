@@ -15,7 +15,9 @@ def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, b_gate: Optional[Tenso
     x [..., dim] fp32, bf16 or fp16 on the GPU; weights [hidden, dim] and biases [hidden] (each optional) in its type.
     activation: silu, gelu (exact), relu, sigmoid or none.  Any number of rows, one included; x and the weights are
     read in place when their rows are 16-byte aligned (dim a multiple of 8, or 4 in fp32), and copied otherwise.
-    fp32 products are fp32 throughout; 16-bit ones accumulate in fp32 and round once.  Differentiable once in all five
+    fp32 products are fp32 throughout; 16-bit ones accumulate in fp32 and round once.  The 16-bit backward also rounds the
+    gradients of the two projections, which its products read (in fp16 within a range of their own: it neither overflows nor
+    loses small gradients there).  Differentiable once in all five
     tensors: fp32 keeps both projections for it (8 bytes a hidden value), 16-bit types keep only their inputs.
     Under torch.autocast all five take its type, as in torch's own products.  Results repeat bit for bit."""
     act = _lib.activation_code("gated_linear", activation)
