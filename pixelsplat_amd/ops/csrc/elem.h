@@ -16,6 +16,9 @@ struct alignas(sizeof(T) * V) Pack { T v[V]; };
 template <typename T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }
 template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }   // round to nearest even
 
+template <typename T> inline constexpr bool kNarrow = false;     // a type with fewer exponents than fp32 has
+template <> inline constexpr bool kNarrow<f16> = true;
+
 // parameters are stored in the tensors' type or in fp32
 template <typename T>
 __device__ __forceinline__ float load_param(const void* p, int is_f32, int64_t i) {

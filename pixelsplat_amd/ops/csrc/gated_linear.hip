@@ -245,9 +245,6 @@ struct StoreGated : NotDone {
   }
 };
 
-template <typename T> constexpr bool kNarrow = false;     // a type whose exponents are fewer than fp32's
-template <> constexpr bool kNarrow<f16> = true;
-
 // fp16: what da and du are multiplied by before they are rounded, and its inverse; powers of two.
 struct Range { float scale, inverse; };
 

@@ -69,8 +69,9 @@ def relative_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, buckets: 
     dim <= 128, at most 2^20 keys, gw <= 512 on grids of more than one row.  The table's gradient takes a workspace of
     queries x keys / 8 bytes a head, twice that on grids of more than one row, and reads the map once a bucket unless
     neighbouring offsets' buckets are near each other.  Differentiable once in q, k, v and table;
-    the gradient of the table is summed over the batch.  16-bit types accumulate in fp32; the
-    backward rounds probabilities and the logits' gradients to them for its products.  Results repeat bit for bit."""
+    the gradient of the table is summed over the batch.  16-bit types accumulate in fp32; the backward rounds probabilities
+    and the logits' gradients to them for its products (in fp16 within a range of their own: they neither overflow nor lose
+    small values there).  Results repeat bit for bit."""
     return _lib.binding().relative_attention(q, k, v, table, buckets, key_mask, scale, query_start)
 
 

@@ -83,3 +83,80 @@ def test_gated_infinities_stay_in_their_row(gpu_device):
         keep = torch.ones(200, dtype=torch.bool, device=gpu_device)
         keep[[7, 150]] = False
         assert torch.isfinite(dx).all() and torch.equal(got[keep], dx[keep]) and not torch.isfinite(got[~keep]).any()
+
+
+def attention_case(dev, heads, grid, dim, queries, start, masked, q_size, k_size, v_size, do_size, grow=0, seed=0):
+    """fp16 tensors of the given sizes; grow: v and do rise by that many powers of two along the tokens."""
+    from pixelsplat_amd.ops import relative_bucket_count, relative_buckets
+
+    g = torch.Generator().manual_seed(seed)
+    n = grid[0] * grid[1]
+    nq = queries or n
+    t = lambda m, size: (torch.randn((2, heads, m, dim), generator=g) * size)  # noqa: E731
+    rise = lambda m: torch.exp2(grow * (torch.arange(m) / m - 1))[:, None]  # noqa: E731
+    q, k, v, do = t(nq, q_size), t(n, k_size), t(n, v_size) * rise(n), t(nq, do_size) * rise(nq)
+    table = 0.3 * torch.randn((relative_bucket_count(grid, 8), heads), generator=g)
+    mask = torch.rand((2, n), generator=g) < 0.7 if masked else None
+    half = [x.half().to(dev) for x in (q, k, v)]
+    return [*half, table.to(dev)], relative_buckets(grid, 8, device=dev), None if mask is None else mask.to(dev), start, \
+        do.half().to(dev)
+
+
+# heads, grid, dim, queries, first query, masked, sizes of q, k, v and do, growth
+T5 = 2.0 ** -5
+BEYOND = [(2, (2, 2), 64, None, 0, False, 0.1, 0.005, 100.0, 1000.0, 0),
+          (1, (3, 40), 32, None, 0, True, 0.05, 0.005, 200.0, 1000.0, 0),
+          (2, (1, 500), 128, 300, 100, False, 0.02, 0.01, 1500.0, 2000.0, 12)]
+BELOW = [(2, (16, 16), 64, None, 0, False, T5, 32.0, 1.0, 2.0 ** -18, 0),
+         (1, (40, 50), 32, None, 0, True, 32.0, T5, 1.0, 2.0 ** -14, 0),
+         (1, (1, 6000), 64, 100, 3000, False, T5, 32.0, 1.0, 2.0 ** -10, 6),
+         (2, (9, 30), 20, 33, 5, True, 32.0, T5, 1.0, 2.0 ** -16, 10),
+         (1, (1, 40000), 16, 300, 20000, False, 1.0, 1.0, 1.0, 1.0, 0)]
+
+
+@pytest.mark.parametrize("case", BEYOND + BELOW, ids=str)
+def test_attention_factors_of_any_size(gpu_device, case):
+    """ds beyond 65504 and where fp16 has few bits, also rising along what is summed; p of a hundred thousandth."""
+    from pixelsplat_amd.ops import relative_attention
+    from tests.test_ops_relative_attention_gpu import bounds
+
+    t, buckets, mask, start, do = attention_case(gpu_device, *case)
+    leaves = [x.requires_grad_() for x in t]
+    call = lambda: torch.autograd.grad(  # noqa: E731
+        relative_attention(*leaves, buckets, key_mask=mask, query_start=start), leaves, do)
+    grads = call()
+    assert all(torch.equal(x, y) for x, y in zip(grads, call()))
+    scale = t[0].shape[3] ** -0.5
+    _, want, _, e = bounds(t, buckets, mask, start, do, scale, torch.float16)
+    qd, kd, vd, td = (x.detach().double() for x in t)
+    ds = R.relative_attention(qd, kd, vd, td, buckets, mask, scale, start, do.double())[2]["ds"].abs()
+    if case in BEYOND:
+        assert ds.max() > 66000
+    if mask is not None:
+        kd = kd * mask[:, None, :, None]
+    # what `bounds` allows for subnormal factors, 2^-24, becomes 2^-38 of the row's or column's largest (p: of 1)
+    for i, (top, other) in enumerate(((ds.amax(3, keepdim=True), kd), (ds.amax(2, keepdim=True).transpose(2, 3), qd))):
+        e[i] = e[i] + scale * (2.0 ** -38 * top - TINY) * other.abs().sum(2, keepdim=True)
+    e[2] = e[2] + (2.0 ** -38 - TINY) * do.double().abs().sum(2, keepdim=True)
+    for name, got, w, bound in zip(("dq", "dk", "dv", "dtable"), grads, want, e):
+        assert name == "dtable" or w.abs().max() < 65000, "the case asks for more than fp16 holds"
+        R.within(got, w, bound, name)
+
+
+def test_attention_infinities_stay_in_their_row(gpu_device):
+    """An infinite and a NaN gradient leave the other queries' dq as it was."""
+    from pixelsplat_amd.ops import relative_attention
+
+    for case in (BEYOND[1], BELOW[1]):
+        t, buckets, mask, start, do = attention_case(gpu_device, *case)
+        q = t[0].requires_grad_()
+        call = lambda d: torch.autograd.grad(  # noqa: E731
+            relative_attention(*t, buckets, key_mask=mask, query_start=start), q, d)[0]
+        want = call(do)
+        bad = do.clone()
+        bad[0, 0, 5, 3], bad[1, 0, 70, 0] = float("inf"), float("nan")
+        got = call(bad)
+        keep = torch.ones(q.shape[:3], dtype=torch.bool, device=gpu_device)
+        keep[0, 0, 5] = keep[1, 0, 70] = False
+        assert torch.isfinite(want).all() and torch.equal(got[keep], want[keep])
+        assert not torch.isfinite(got[0, 0, 5]).any() and not torch.isfinite(got[1, 0, 70]).any()
