@@ -64,7 +64,7 @@ struct Args {
   // forward
   void* out;                      // [batch][nq][heads][dim]
   float* o32;                     // the same in fp32 or NULL
-  float* stats;                   // [2][batch heads][nq_pad] or NULL: maximum (log2, or up to 8 less; +inf: no keys), 1 / sum (0)
+  float* stats;                   // [2][batch heads][nq_pad] or NULL: maximum (log2, or up to 15 less; +inf: no keys), 1 / sum (0)
   float *part_o, *part_ml;        // [splits][batch heads nq][dim], [..][2]
   int join_lanes;                 // threads that share a row's splits
   // backward
@@ -300,6 +300,7 @@ __global__ void __launch_bounds__(256) spread_table_kernel(int heads, int offset
 template <typename T, int DP, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64, DP == 128 && (sizeof(T) == 4 || WAVES == 1) ? 1 : 2) attention_forward_kernel(Args p) {
   constexpr int PITCH = DP * sizeof(T), ROWS = kRows<T>, SUBS = ROWS / 32, KF = DP / kFragK<T>, PF = 32 / kFragK<T>;
+  constexpr float kLift = kNarrow<T> ? 7.f : 0.f;
   typedef Lds<T, DP, WAVES> L;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, hi = lane >> 5;
@@ -379,9 +380,11 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 128 && (sizeof(T) == 4 || WA
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
     top = fmaxf(top, __shfl_xor(top, 32));
-    // A new maximum: what there is shrinks.  Not for every one: terms of up to 2^8 are as exact as those of up to 1.
-    if (__any(top > m + 8.f)) {
-      const float nm = fmaxf(m, top);
+    // A new maximum: what there is shrinks.  Not for every one: terms of up to 2^8 are as exact as those of up to 1.  In fp16,
+    // which ends at 2^-24 and 2^16, the largest term is 2^7 .. 2^15: a term 2^-25 of it is lost, and 2^18 keys of those are
+    // a hundredth of the result; 2^-32 of it is not missed.
+    if (__any(top > m + (8.f + kLift))) {
+      const float nm = fmaxf(m, top - kLift);
       const float by = __builtin_amdgcn_exp2f(m - (nm == -kInf ? 0.f : nm));
       m = nm;
       l *= by;

@@ -160,3 +160,27 @@ def test_attention_infinities_stay_in_their_row(gpu_device):
         keep[0, 0, 5] = keep[1, 0, 70] = False
         assert torch.isfinite(want).all() and torch.equal(got[keep], want[keep])
         assert not torch.isfinite(got[0, 0, 5]).any() and not torch.isfinite(got[1, 0, 70]).any()
+
+
+@pytest.mark.parametrize("queries", [1, 40])
+@pytest.mark.parametrize("below", [17.5, 20.0])
+def test_attention_terms_far_below_the_largest(gpu_device, below, queries):
+    """One key ahead of 2^18 others that are e^-17.5 (2^-25) or less each and together a good part of the result.  A term
+    and what its rounding leaves are off by 2^-32 of the largest term at most where they are subnormal."""
+    from pixelsplat_amd.ops import relative_attention, relative_buckets
+    from tests.test_ops_relative_attention_gpu import bounds
+
+    n = 1 << 18
+    q = torch.zeros((1, 1, queries, 16), dtype=torch.float16, device=gpu_device)
+    k, v = torch.zeros((2, 1, 1, n, 16), dtype=torch.float16, device=gpu_device)
+    q[..., 0] = 1
+    k[..., 777, 0] = below
+    v[:] = 1
+    v[..., 777, :] = 0
+    table = torch.zeros((8, 1), dtype=torch.float16, device=gpu_device)
+    buckets = relative_buckets((1, n), 8, device=gpu_device)
+    ref, _, e, _ = bounds([q, k, v, table], buckets, None, 0, torch.zeros_like(q), 1.0, torch.float16)
+    bound = e + (2.0 ** -31 - TINY) * v.double().abs().sum(2, keepdim=True)
+    assert (bound < ref / 2).all()                       # a lost sum would be seen
+    R.within(relative_attention(q, k, v, table, buckets, scale=1.0), ref, bound, "out")
+    R.within(relative_attention(q.requires_grad_(), k, v, table, buckets, scale=1.0), ref, bound, "out in training")
