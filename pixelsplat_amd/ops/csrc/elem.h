@@ -86,9 +86,9 @@ __device__ __forceinline__ float act_slope(float z, float* value) {
     return fmaf(z * 0.39894228040143268f, bell, cdf);
   }
   if constexpr (ACT == ACT_SIGMOID) {
-    const float s = sigmoid_f32(z);
-    *value = s;
-    return s * (1.f - s);
+    const float e = __expf(-fabsf(z)), r = 1.f / (1.f + e);      // s (1 - s) would lose 1 - s where s is near 1
+    *value = z < 0.f ? e * r : r;
+    return e * r * r;
   }
   *value = z;
   return 1.f;
