@@ -12,8 +12,9 @@
 // alternating runs of 32, so that the wave that holds a also holds u and the activation is its epilogue: neither
 // projection reaches memory.
 //
-// 16384 x 1024 -> 4096 in bf16, silu: forward 335 us (275 GFLOP, 820 TFLOP/s; its copies alone 246, its matrix instructions
-// alone 249), da and du 395, dx 335, both weight gradients 322.  One token of it: 4.4 us for 17 MB of weights.
+// 16384 x 1024 -> 4096 in bf16, silu: forward 342 us (275 GFLOP, 800 TFLOP/s; the fastest of 23 passes 322: its copies alone
+// 246, its matrix instructions alone 249), da and du 417, dx 350, both weight gradients 331.  One token of it: 4.4 us for 17 MB of
+// weights.
 //
 // What the backward needs of a and u: fp32 tensors keep both (8 bytes a hidden value, against 4 D flop at 150
 // TFLOP/s); 16-bit tensors compute them again (the products are 8 times as fast, and keeping them rounded to 16 bits

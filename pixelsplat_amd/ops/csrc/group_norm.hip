@@ -3,13 +3,14 @@
 //   dz = dy act'(z);  d_beta = sum dz;  d_gamma = sum dz xh;
 //   dx = rstd (gamma dz - mean(gamma dz) - xh mean(gamma dz xh)).
 //
-// Bound by memory.  Two forms:
+// Bound by memory in the statistics and in fp32, by the activation's vector instructions in 16 bits.  Two forms:
 //  * one block per (sample, group) that keeps the whole group in registers (x read once, y written once): one launch,
 //    for groups of up to kHeld vectors a thread whose row segments are at least 32 bytes;
 //  * chunks of rows: one pass writes sums per (sample, chunk, group), a second folds the sums of its sample and
 //    writes y.  The second pass takes the chunks in the opposite order, so that what the first read last is still in
-//    the 256 MB memory-side cache.  14 x 65536 rows of 256 in bf16 (470 MB), 32 groups, gelu: sums 130 us (3.6 TB/s),
-//    y 212 (4.4), gradient's sums 255 (3.7), dx 278 (5.1, some of it from that cache).  Passing a few samples at a time
+//    the 256 MB memory-side cache.  14 x 65536 rows of 256 in bf16 (470 MB), 32 groups, gelu: sums 132 us (3.6 TB/s),
+//    y 209 (166 of them its 22 vector instructions an element, two transcendental), gradient's sums 257 (29 an element:
+//    208), dx 275 (29: 211).  Passing a few samples at a time
 //    through both passes, all of them from the cache, took 1716 us: launches that small do not fill the memory.
 // Sums over x and x^2 are held in 64 bits: E[x^2] - mean^2 then needs no pivot, whatever the mean is, and the double
 // adds hide under the loads.  The backward's sums are fp32 within a thread (at most 256 rows) and 64 bits across threads and

@@ -34,8 +34,8 @@
 //
 // Bound by the matrix instructions in fp32, by the vector instructions of the softmax in 16 bits, by the keys' and
 // values' bytes for a few queries, which split the keys over blocks and join their partial results.  2 x 8 heads of 64 x 64
-// tokens of 64 in bf16: forward 173 us, dq and the table's rows 250, dk and dv 197, the table's joins 45.  14 x 4 heads of
-// 16 x 16 tokens of 128 in fp32: 35, 57, 53 and 23.  One query of 4 x 8 heads over 16384 keys of 64 in bf16: 27 us, 5 TB/s.
+// tokens of 64 in bf16: forward 176 us, dq and the table's rows 254, dk and dv 201, the table's joins 45.  14 x 4 heads of
+// 16 x 16 tokens of 128 in fp32: 35, 58, 53 and 23.  One query of 4 x 8 heads over 16384 keys of 64 in bf16: 28 us, 4.8 TB/s.
 #include "mfma_tile.h"
 #include "pixelsplat_ops.h"
 
