@@ -344,3 +344,17 @@ def test_attention_workspace_without_the_tables_gradient(lib):
         assert 0 < size(side, 2) <= 2 * side * side * 64 * 4 * 3 * 16 + (1 << 20), side      # parts of up to 16 splits
         assert size(side, 2) < size(side, 1)
     assert size(512, 2) <= 16 * size(128, 2) and size(512, 1) > 128 * size(128, 1)
+
+
+def test_attention_backward_wants_the_workspace_of_what_it_computes(lib):
+    """The size without the table's gradient is refused where that gradient is asked for."""
+    from pixelsplat_amd.ops import _lib
+    p, s = 4096, (C.c_int64 * 3)(96, 8, 24)          # an address that is never followed
+    d = _lib.PsRelativeAttentionDesc(batch=2, heads=1, queries=6, query_start=0, grid_h=2, grid_w=3, dim=8, dtype=2, buckets=5,
+                                     table_f32=0, scale=0.3, reserved=0, q_strides=s, k_strides=s, v_strides=s, do_strides=s,
+                                     mask_stride=6)
+    small, full = (lib.ps_relative_attention_workspace_bytes(C.byref(d), what) for what in (2, 1))
+    assert 0 < small < full
+    for n in (small, full - 1):
+        assert lib.ps_relative_attention_backward(C.byref(d), p, p, p, None, p, p, p, p, p, p, p, p, p, p, n, None) == -2
+    assert lib.ps_relative_attention_backward(C.byref(d), p, p, p, None, p, p, p, p, p, p, p, p, None, p, small - 1, None) == -2

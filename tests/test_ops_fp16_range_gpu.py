@@ -186,3 +186,39 @@ def test_attention_terms_far_below_the_largest(gpu_device, below, queries):
     assert (bound < ref / 2).all()                       # a lost sum would be seen
     R.within(relative_attention(q, k, v, table, buckets, scale=1.0), ref, bound, "out")
     R.within(relative_attention(q.requires_grad_(), k, v, table, buckets, scale=1.0), ref, bound, "out in training")
+
+
+def test_ranges_in_a_graph_and_on_another_stream(gpu_device):
+    """A captured training step of both operators, replayed with gradients of other sizes: the range is chosen in each replay."""
+    from pixelsplat_amd.ops import gated_linear, relative_attention
+
+    t, buckets, mask, start, do = attention_case(gpu_device, 2, (6, 20), 32, None, 0, True, 0.1, 0.1, 1.0, 1.0)
+    g = torch.Generator().manual_seed(4)
+    x = (torch.randn((300, 64), generator=g) * 0.01).half().to(gpu_device)
+    w = (torch.randn((96, 64), generator=g) * 0.01).half().to(gpu_device)
+    b = torch.full((96,), 50.0, device=gpu_device).half()
+    dh = torch.randn((300, 96), generator=g).half().to(gpu_device)
+    leaves = [p.requires_grad_() for p in (*t, x, w)]
+
+    def step():
+        y, h = relative_attention(*leaves[:4], buckets, key_mask=mask), gated_linear(x, w, w, b, b)
+        return [*torch.autograd.grad(y, leaves[:4], do), *torch.autograd.grad(h, leaves[4:], dh)]
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i, size in enumerate((1.0, 2.0 ** -14, 800.0, 2.0 ** -10, 1.0, 800.0)):
+        with torch.no_grad():
+            do.copy_((torch.randn(do.shape, generator=g) * size).half())
+            dh.copy_((torch.randn(dh.shape, generator=g) * size).half())
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = step()
+        assert all(torch.equal(p, q) and torch.isfinite(p).all() for p, q in zip(out, eager)), (i, size)
